@@ -1,0 +1,523 @@
+"""The operators a quantized model answers with, measured: products of a few tokens with 4-bit
+packed weights, block tables planned on the GPU, keys and values appended to an 8-bit block
+cache, and attention over that cache.
+
+`listed()` are the measured cases, `draw()` gives more of the same ranges.  Where `own` is
+false `run()` computes the operators from elementary torch operations in 32 bits; where it is
+true it calls the framework.
+
+Data formats (the framework's):
+  weight_packed      int32 [N, K/8], code of column k in bits 4*(k%8) of word k/8, stored + 8
+  weight_zero_point  int32 [ceil(N/8), groups], the same packing along the rows
+  cache.key          [blocks, kv heads, block size, head dim]  8-bit codes
+  cache.value        [blocks, kv heads, head dim, block size]  8-bit codes
+  cache.key_scale, cache.value_scale   fp32 [blocks, kv heads]
+"""
+import math
+import sys
+from pathlib import Path
+
+import torch
+
+own = False
+
+HEADS, KV_HEADS = 32, 8  # the attention of the 4096-wide model whose weights bench.py compresses
+DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16}
+CODES = {"fp8": torch.float8_e4m3fn, "int8": torch.int8}
+CODE_MAX = {"fp8": 448.0, "int8": 127.5}  # half the range of the codes: max|x| / this is the scale
+EPS = torch.finfo(torch.float32).eps  # smallest scale
+
+
+def _package():
+    """the framework's entry points, imported where they are called"""
+    at = str(Path(__file__).resolve().parent.parent / "compressed-tensors_amd")
+    if at not in sys.path:
+        sys.path.insert(0, at)
+    from compressed_tensors_amd import linear, modeling
+
+    return linear, modeling
+
+
+# ------------------------------------------------------------------------------------ cases
+def listed():
+    return [
+        # one token through a square projection: the smallest product of a decode step, where latency counts
+        {"name": "linear-1x4096x4096", "op": "linear", "m": 1, "n": 4096, "k": 4096, "group": 128,
+         "asym": False, "bias": False, "dtype": "bf16"},
+        # a few tokens, a width that is no multiple of any tile, groups of 32 with zero points
+        {"name": "linear-5x1001x4160", "op": "linear", "m": 5, "n": 1001, "k": 4160, "group": 32,
+         "asym": True, "bias": True, "dtype": "bf16"},
+        # a batch of 16 decoding requests through the fused gate and up projections
+        {"name": "linear-16x28672x4096", "op": "linear", "m": 16, "n": 28672, "k": 4096, "group": 128,
+         "asym": True, "bias": False, "dtype": "bf16"},
+        # a batch of 64 through the down projection
+        {"name": "linear-64x4096x14336", "op": "linear", "m": 64, "n": 4096, "k": 14336, "group": 128,
+         "asym": False, "bias": True, "dtype": "fp16"},
+        # a serving step: every request gains one token, blocks of 64 tokens
+        {"name": "append-48x1", "op": "append", "requests": 48, "context": 2000, "new": 1, "block": 64,
+         "head_dim": 128, "codes": "fp8", "dtype": "bf16"},
+        # prompts of odd lengths written in one call, into blocks begun by earlier tokens
+        {"name": "append-3x4001", "op": "append", "requests": 3, "context": 75, "new": 4001, "block": 32,
+         "head_dim": 128, "codes": "int8", "dtype": "fp16"},
+        # drafted tokens checked in one pass for three short requests: the smallest attention call
+        {"name": "attend-3x5-777", "op": "attend", "requests": 3, "context": 777, "new": 5, "block": 16,
+         "head_dim": 64, "heads": 8, "kv_heads": 2, "codes": "fp8", "dtype": "bf16"},
+        # a decoding batch of ragged lengths up to 4096
+        {"name": "attend-64x1-4096", "op": "attend", "requests": 64, "context": 4096, "new": 1, "block": 64,
+         "head_dim": 128, "heads": HEADS, "kv_heads": KV_HEADS, "codes": "fp8", "dtype": "bf16"},
+        # few requests with long contexts: one row of queries against up to 32 768 keys
+        {"name": "attend-6x1-32768", "op": "attend", "requests": 6, "context": 32768, "new": 1, "block": 32,
+         "head_dim": 128, "heads": HEADS, "kv_heads": KV_HEADS, "codes": "int8", "dtype": "fp16"},
+        # chunks of prompts, 2000 new tokens each, behind contexts up to 2000
+        {"name": "attend-2x2000-4000", "op": "attend", "requests": 2, "context": 4000, "new": 2000, "block": 64,
+         "head_dim": 128, "heads": HEADS, "kv_heads": KV_HEADS, "codes": "fp8", "dtype": "bf16"},
+        # a small serving step's bookkeeping
+        {"name": "plan-24", "op": "plan", "requests": 24, "width": 64, "block": 64, "prompt": 1},
+        # a large one: a thousand requests, some ended, some new with prompts
+        {"name": "plan-1000", "op": "plan", "requests": 1000, "width": 257, "block": 32, "prompt": 1900},
+    ]
+
+
+def _log(rng, low, high):
+    return int(round(math.exp(rng.uniform(math.log(low), math.log(high)))))
+
+
+def draw(rng):
+    op = rng.choice(["linear", "linear", "append", "attend", "attend", "plan"])
+    dtype = rng.choice(["bf16", "fp16"])
+    codes = rng.choice(["fp8", "int8"])
+    block = rng.choice([16, 32, 64, 128])
+    if op == "linear":
+        group = rng.choice([32, 64, 128])
+        m = _log(rng, 1, 64)
+        n = _log(rng, 512, 14336)
+        k = group * max(1, _log(rng, 512, min(14336, 64 * 4096 * 14336 // (m * n))) // group)
+        return {"op": "linear", "m": m, "n": n, "k": k, "group": group, "asym": rng.random() < 0.5,
+                "bias": rng.random() < 0.5, "dtype": dtype}
+    head_dim = rng.choice([64, 128])
+    if op == "append":
+        if rng.random() < 0.5:
+            requests, new = _log(rng, 1, 128), 1
+        else:
+            requests, new = _log(rng, 1, 8), _log(rng, 2, 1100)
+        return {"op": "append", "requests": requests, "context": _log(rng, 1, 2000), "new": new,
+                "block": block, "head_dim": head_dim, "codes": codes, "dtype": dtype}
+    if op == "attend":
+        kv_heads = rng.choice([1, 2, 8])
+        heads = kv_heads * rng.choice([1, 2, 4, 8] if kv_heads > 1 else [1, 4, 7, 16])
+        kind = rng.random()
+        if kind < 0.5:
+            requests, new, context = _log(rng, 1, 64), 1, _log(rng, 1, 8192)
+            context = max(1, min(context, 64 * 4096 // requests))
+        elif kind < 0.75:
+            requests, new = _log(rng, 1, 16), rng.randint(2, 9)
+            context = new + _log(rng, 1, 8192)
+        else:
+            requests, new = rng.randint(1, 2), _log(rng, 10, 1000)
+            context = new + _log(rng, 1, 2000)
+        return {"op": "attend", "requests": requests, "context": context, "new": new, "block": block,
+                "head_dim": head_dim, "heads": heads, "kv_heads": kv_heads, "codes": codes, "dtype": dtype}
+    return {"op": "plan", "requests": _log(rng, 1, 1000), "width": _log(rng, 64, 257), "block": block,
+            "prompt": _log(rng, 1, 1900)}
+
+
+def _lengths(case):
+    """tokens each request has once the new ones are in: from 2/3 of `context` up to all of it,
+    the first the longest; never fewer than its new tokens"""
+    context, new = case["context"], case["new"]
+    return [max(new, context - (i * 577) % (context // 3 + 1)) for i in range(case["requests"])]
+
+
+def _append_counts(case):
+    """(tokens before, new tokens) of each request of an append case: ragged, one token each
+    where new == 1"""
+    before = [max(0, case["context"] - (i * 577) % (case["context"] // 2 + 1)) for i in range(case["requests"])]
+    new = [max(1, case["new"] - (i * 379) % (case["new"] // 2 + 1)) for i in range(case["requests"])]
+    return before, new
+
+
+def _plan_counts(case):
+    """(tokens before, new tokens) of each request of a planning case: every 16th has ended (-1),
+    every 16th is new with a prompt, the others gain one token"""
+    cap = case["width"] * case["block"]
+    before, new = [], []
+    for i in range(case["requests"]):
+        if i % 16 == 5:
+            before.append(1 + (i * 977) % (cap - 1))
+            new.append(-1)
+        elif i % 16 == 9:
+            before.append(0)
+            new.append(min(cap, max(1, case["prompt"] - (i * 131) % (case["prompt"] // 2 + 1))))
+        else:
+            before.append((i * 977) % (cap - 1))
+            new.append(1)
+    return before, new
+
+
+def work(case):
+    op = case["op"]
+    if op == "linear":
+        m, n, k, groups = case["m"], case["n"], case["k"], case["k"] // case["group"]
+        moved = n * k // 2 + n * groups * 2 + 2 * m * k + 2 * m * n
+        moved += (n + 7) // 8 * 4 * groups if case["asym"] else 0
+        moved += 2 * n if case["bias"] else 0
+        return {"bytes": moved, "flops": 2 * m * n * k}
+    if op == "append":
+        before, new = _append_counts(case)
+        tokens = sum(new)
+        values = 2 * tokens * KV_HEADS * case["head_dim"]
+        touched = sum((b + t - 1) // case["block"] - b // case["block"] + 1 for b, t in zip(before, new))
+        return {"bytes": values * 3 + tokens * 8 + touched * KV_HEADS * 2 * 8, "flops": 4 * values}
+    if op == "attend":
+        lens, new, d = _lengths(case), case["new"], case["head_dim"]
+        pairs = sum(new * (n - new) + new * (new + 1) // 2 for n in lens)
+        blocks = sum(-(-n // case["block"]) for n in lens)
+        moved = 2 * sum(lens) * case["kv_heads"] * d + blocks * (4 + 8 * case["kv_heads"])
+        moved += 2 * 2 * len(lens) * new * case["heads"] * d
+        return {"bytes": moved, "flops": 4 * pairs * case["heads"] * d}
+    before, new = _plan_counts(case)
+    tokens = sum(t for t in new if t > 0)
+    pool = _pool(case)
+    return {"bytes": 2 * 4 * (case["requests"] * (case["width"] + 1) + pool) + 4 * case["requests"] + 8 * tokens,
+            "flops": 0}
+
+
+def _pool(case):
+    """blocks of the pool a planning case draws on: what its requests hold and what they will need"""
+    before, new = _plan_counts(case)
+    bs = case["block"]
+    return sum(-(-(b + max(t, 0)) // bs) for b, t in zip(before, new)) + 7
+
+
+# ---------------------------------------------------------------------------------- inputs
+def _generator(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(int(seed))
+    return g
+
+
+def _randn(g, *shape):
+    return torch.randn(*shape, generator=g, device="cuda", dtype=torch.float32)
+
+
+def _ints(g, low, high, *shape):
+    return torch.randint(low, high, shape, generator=g, device="cuda", dtype=torch.int32)
+
+
+def _device_ints(values, dtype=torch.int32):
+    return torch.tensor(values, dtype=dtype, device="cuda")
+
+
+def _make_cache(case, kv_heads, blocks, g):
+    """a pool in use: codes of normally distributed keys and values, scales that differ from
+    block to block"""
+    bs, d, kind = case["block"], case["head_dim"], case["codes"]
+    tensors = []
+    for shape in ((blocks, kv_heads, bs, d), (blocks, kv_heads, d, bs)):
+        x = _randn(g, *shape) * (CODE_MAX[kind] / 4.0)
+        x = x.clamp_(-448.0, 448.0) if kind == "fp8" else x.round_().clamp_(-128.0, 127.0)
+        tensors.append(x.to(CODES[kind]))
+        del x
+    for mean in (1.0, 0.6):  # values are smaller than keys
+        tensors.append(mean * 4.0 / CODE_MAX[kind] * (0.5 + torch.rand(blocks, kv_heads, generator=g, device="cuda")))
+    return tuple(tensors)
+
+
+def _tables(lens, bs, g, spare=3):
+    """a block table for requests of these lengths: blocks scattered over the pool, -1 behind"""
+    need = [-(-n // bs) for n in lens]
+    width, total = max(max(need), 1), sum(need)
+    order = torch.randperm(total + spare, generator=g, device="cuda").to(torch.int32)
+    table = torch.full((len(lens), width), -1, dtype=torch.int32, device="cuda")
+    rows = torch.repeat_interleave(torch.arange(len(lens)), torch.tensor(need))
+    cols = torch.cat([torch.arange(n) for n in need])
+    table[rows.cuda(), cols.cuda()] = order[:total]
+    return table, total + spare
+
+
+def prepare(case, seed):
+    g = _generator(seed)
+    state = {"case": dict(case)}
+    op = case["op"]
+    if op == "linear":
+        dt = DTYPES[case["dtype"]]
+        m, n, k = case["m"], case["n"], case["k"]
+        groups = k // case["group"]
+        state["x"] = _randn(g, m, k).to(dt)
+        # every code is as likely as in a quantized normal weight: words of four-bit draws
+        words = torch.zeros(n, k // 8, dtype=torch.int32, device="cuda")
+        zeros = torch.zeros((n + 7) // 8, groups, dtype=torch.int32, device="cuda")
+        for i in range(8):
+            code = (_randn(g, n, k // 8) * 2.7 + 8.0).round_().clamp_(0, 15).to(torch.int32)
+            words |= code << (4 * i)
+            if case["asym"]:
+                zeros |= _ints(g, 4, 13, (n + 7) // 8, groups) << (4 * i)
+        state["packed"] = words
+        state["scale"] = ((0.5 + torch.rand(n, groups, generator=g, device="cuda")) * 0.01).to(dt)
+        state["zero"] = zeros if case["asym"] else None
+        state["bias"] = _randn(g, n).to(dt) if case["bias"] else None
+        return state
+    if op == "append":
+        before, new = _append_counts(case)
+        dt, bs = DTYPES[case["dtype"]], case["block"]
+        table, blocks = _tables([b + t for b, t in zip(before, new)], bs, g)
+        state["cache"] = _make_cache(case, KV_HEADS, blocks, g)
+        at = torch.cat([torch.arange(b, b + t) for b, t in zip(before, new)]).cuda()
+        rows = torch.repeat_interleave(torch.arange(len(new)), torch.tensor(new)).cuda()
+        state["slots"] = table[rows, at // bs].long() * bs + at % bs
+        state["touched"] = sum((b + t - 1) // bs - b // bs + 1 for b, t in zip(before, new))
+        # some channels of real keys are far larger than the others
+        spread = torch.exp(0.5 * _randn(g, 1, KV_HEADS, case["head_dim"]))
+        state["k"] = (_randn(g, sum(new), KV_HEADS, case["head_dim"]) * spread).to(dt)
+        state["v"] = (_randn(g, sum(new), KV_HEADS, case["head_dim"]) * 0.6).to(dt)
+        return state
+    if op == "attend":
+        lens = _lengths(case)
+        state["table"], blocks = _tables(lens, case["block"], g)
+        state["cache"] = _make_cache(case, case["kv_heads"], blocks, g)
+        state["lens"] = _device_ints(lens)
+        state["starts"] = _device_ints([i * case["new"] for i in range(len(lens) + 1)])
+        state["max_seq"], state["max_query"] = max(lens), case["new"]
+        state["q"] = _randn(g, len(lens) * case["new"], case["heads"], case["head_dim"]).to(DTYPES[case["dtype"]])
+        return state
+    before, new = _plan_counts(case)
+    bs, pool = case["block"], _pool(case)
+    need = [-(-b // bs) for b in before]
+    order = torch.randperm(pool, generator=g, device="cuda").to(torch.int32)
+    table = torch.full((case["requests"], case["width"]), -1, dtype=torch.int32, device="cuda")
+    rows = torch.repeat_interleave(torch.arange(len(need)), torch.tensor(need)).cuda()
+    cols = torch.cat([torch.arange(n) for n in need]).cuda()
+    table[rows, cols] = order[: sum(need)]
+    free = torch.full((pool,), -1, dtype=torch.int32, device="cuda")
+    free[: pool - sum(need)] = order[sum(need):]
+    state.update(table=table, free=free, lens=_device_ints(before), new=_device_ints(new),
+                 num_free=_device_ints([pool - sum(need)]), total=sum(t for t in new if t > 0))
+    return state
+
+
+# ------------------------------------------------------------------------------ plain forms
+def _unpack4(words, dim):
+    """the eight 4-bit codes (0 ... 15) of each word, laid out along `dim`"""
+    shifts = torch.arange(0, 32, 4, device=words.device, dtype=torch.int32)
+    codes = (words.unsqueeze(-1) >> shifts) & 15
+    if dim == 1:
+        return codes.flatten(1)
+    return codes.permute(0, 2, 1).flatten(0, 1)
+
+
+def _plain_linear(s):
+    n, k, group = s["case"]["n"], s["case"]["k"], s["case"]["group"]
+    q = _unpack4(s["packed"], 1).view(n, k // group, group) - 8
+    if s["zero"] is not None:
+        q = q - (_unpack4(s["zero"], 0)[:n] - 8).unsqueeze(-1)
+    w = (q.float() * s["scale"].float().unsqueeze(-1)).view(n, k)
+    y = s["x"].float() @ w.t()
+    if s["bias"] is not None:
+        y = y + s["bias"].float()
+    return y.to(s["x"].dtype)
+
+
+def _encode(x, scale, kind):
+    """codes of x / scale; saturating"""
+    x = x / scale
+    if kind == "fp8":
+        return x.clamp(-448.0, 448.0).to(torch.float8_e4m3fn)
+    return x.clamp(-128.0, 127.0).round().to(torch.int8)
+
+
+def _plain_append(s):
+    kind, bs = s["case"]["codes"], s["case"]["block"]
+    key, value, key_scale, value_scale = s["cache"]
+    slots = s["slots"]
+    block, offset = slots // bs, slots % bs
+    first = torch.ones_like(block, dtype=torch.bool)
+    first[1:] = block[1:] != block[:-1]
+    at = first.long().cumsum(0) - 1  # which of the touched blocks a token goes to
+    blocks = torch.zeros(s["touched"], dtype=torch.long, device=block.device).scatter_(0, at, block)
+    start = torch.full_like(blocks, bs).scatter_reduce_(0, at, offset, "amin")  # first new position
+    fresh = (start == 0).view(-1, 1)
+    ages = torch.arange(bs, device=block.device) < start.view(-1, 1)  # positions filled before
+    out = []
+    for x, codes, scale, transposed in ((s["k"], key, key_scale, False), (s["v"], value, value_scale, True)):
+        x = x.float()
+        peak = torch.zeros(s["touched"], x.shape[1], device=x.device)
+        peak.scatter_reduce_(0, at.view(-1, 1).expand(-1, x.shape[1]), x.abs().amax(-1), "amax")
+        fits = (peak / torch.full_like(peak, CODE_MAX[kind])).clamp(min=EPS)  # a true division
+        old = scale[blocks]
+        now = torch.where(fresh, fits, torch.maximum(old, fits))
+        raw = codes.view(torch.uint8)
+        was = raw[blocks].view(codes.dtype).float()
+        again = _encode(was * (old / now).view(*now.shape, 1, 1), 1.0, kind).view(torch.uint8)
+        keep = ages[:, None, None, :] if transposed else ages[:, None, :, None]
+        raw[blocks] = torch.where(keep, again, raw[blocks])
+        new = _encode(x, now[at].unsqueeze(-1), kind).view(torch.uint8)
+        if transposed:
+            raw[block, :, :, offset] = new
+        else:
+            raw[block, :, offset] = new
+        scale[blocks] = now
+        out += [codes, scale]
+    return out
+
+
+def _plain_attend(s):
+    c = s["case"]
+    key, value, key_scale, value_scale = s["cache"]
+    table, lens, new, d = s["table"].long().clamp(min=0), s["lens"], c["new"], c["head_dim"]
+    requests, width = table.shape
+    length, share = width * c["block"], c["heads"] // c["kv_heads"]
+    k = key.view(torch.uint8)[table].view(key.dtype).float() * key_scale[table][..., None, None]
+    k = k.transpose(1, 2).reshape(requests, c["kv_heads"], length, d)
+    q = s["q"].float().view(requests, new, c["kv_heads"], share, d)
+    q = q.permute(0, 2, 1, 3, 4).reshape(requests, c["kv_heads"], new * share, d)
+    score = torch.matmul(q, k.transpose(-1, -2).contiguous()) / math.sqrt(d)
+    del k
+    place = lens.view(-1, 1) - new + torch.arange(new * share, device=lens.device) // share
+    hidden = torch.arange(length, device=lens.device) > place.unsqueeze(-1)
+    score = score.masked_fill(hidden.unsqueeze(1), float("-inf"))
+    top = score.amax(-1, keepdim=True)
+    p = torch.exp(score - torch.where(top == float("-inf"), torch.zeros_like(top), top))
+    del score
+    total = p.sum(-1, keepdim=True)
+    v = value.view(torch.uint8)[table].view(value.dtype).float() * value_scale[table][..., None, None]
+    v = v.permute(0, 2, 1, 4, 3).reshape(requests, c["kv_heads"], length, d)
+    o = torch.matmul(p, v) / torch.where(total == 0, torch.ones_like(total), total)
+    o = o.view(requests, c["kv_heads"], new, share, d).permute(0, 2, 1, 3, 4)
+    return o.reshape(requests * new, c["heads"], d).to(s["q"].dtype)
+
+
+def _plain_plan(s):
+    bs, total = s["case"]["block"], s["total"]
+    lens, table, free, num_free = s["lens"].long(), s["table"], s["free"], s["num_free"].long()
+    ended, add = s["new"] < 0, s["new"].clamp(min=0).long()
+    held = (lens + bs - 1) // bs
+    after = torch.where(ended, torch.zeros_like(lens), lens + add)
+    need = (after + bs - 1) // bs
+    want = torch.where(ended, torch.zeros_like(need), need - held)
+    # the stack of free blocks, what the ended requests held on top of it in request order
+    column = torch.arange(table.shape[1], device=table.device)
+    given_back = ended.unsqueeze(1) & (column < held.unsqueeze(1))
+    above = given_back.flatten().long().cumsum(0) - 1 + num_free
+    stack = torch.where(torch.arange(free.numel(), device=free.device) < num_free, free, torch.full_like(free, -1))
+    stack = torch.cat([stack, stack.new_zeros(1)])  # the last entry takes what does not belong
+    stack.scatter_(0, torch.where(given_back.flatten(), above, torch.full_like(above, free.numel())), table.flatten())
+    size = num_free + given_back.sum()
+    # new blocks in request order from the top of the stack
+    order = want.cumsum(0) - want
+    fresh = (column >= held.unsqueeze(1)) & (column < need.unsqueeze(1)) & ~ended.unsqueeze(1)
+    from_top = size - 1 - (order.unsqueeze(1) + column - held.unsqueeze(1))
+    table = torch.where(fresh, stack[from_top.clamp(0, free.numel() - 1)], table)
+    table = torch.where(ended.unsqueeze(1), torch.full_like(table, -1), table)
+    left = size - want.sum()
+    free = torch.where(torch.arange(free.numel(), device=free.device) < left, stack[:-1], torch.full_like(free, -1))
+    starts = torch.cat([add.new_zeros(1), add.cumsum(0)])
+    token = torch.arange(total, device=lens.device)
+    request = torch.searchsorted(starts, token, right=True) - 1
+    place = lens[request] + token - starts[request]
+    slots = table[request, place // bs].long() * bs + place % bs
+    return [after.int(), starts.int(), slots, table, free, left.int().view(1), torch.zeros_like(s["num_free"])]
+
+
+def run(state):
+    op = state["case"]["op"]
+    if not own:
+        return {"linear": _plain_linear, "append": _plain_append, "attend": _plain_attend, "plan": _plain_plan}[op](state)
+    linear, modeling = _package()
+    if op == "linear":
+        return linear.packed_linear(state["x"], state["packed"], state["scale"], state["zero"], state["bias"])
+    if op == "plan":
+        p = modeling.plan_kv_blocks(state["lens"], state["new"], state["table"], state["free"], state["num_free"],
+                                    block_size=state["case"]["block"], total_tokens=state["total"])
+        return [p.seq_lens, p.query_start, p.slots, p.block_table, p.free_blocks, p.num_free, p.status]
+    cache = modeling.KVBlocks(*state["cache"])
+    if op == "append":
+        modeling.append_kv_blocks(state["k"], state["v"], cache, state["slots"])
+        return [cache.key, cache.key_scale, cache.value, cache.value_scale]
+    return modeling.attend_kv_blocks(state["q"], cache, state["table"], state["lens"], state["starts"],
+                                     max_query=state["max_query"], max_seq=state["max_seq"])
+
+
+# --------------------------------------------------------------------------------- 64 bits
+def _code_values(t):
+    return t.to(torch.float32).to(torch.float64)
+
+
+def _exact_linear(s):
+    n, group = s["case"]["n"], s["case"]["group"]
+    y = torch.zeros(s["x"].shape[0], n, dtype=torch.float64, device="cuda")
+    x = s["x"].double()
+    row = torch.arange(n, device="cuda")
+    for j in range(s["scale"].shape[1]):
+        words = s["packed"][:, j * group // 8:(j + 1) * group // 8].long() & 0xFFFFFFFF
+        part = torch.zeros_like(y)
+        for i in range(8):
+            part += x[:, j * group + i:(j + 1) * group:8] @ ((words >> (4 * i)) & 15).double().t().contiguous()
+        zero = 8.0
+        if s["zero"] is not None:
+            packed = s["zero"][row // 8, j].long() & 0xFFFFFFFF
+            zero = ((packed >> (4 * (row % 8))) & 15).double()
+        part -= x[:, j * group:(j + 1) * group].sum(1, keepdim=True) * zero
+        y += part * s["scale"][:, j].double()
+    return y if s["bias"] is None else y + s["bias"].double()
+
+
+def _nearest_e4m3(x):
+    """the nearest e4m3 value (ties to the even mantissa), saturating at 448"""
+    x = x.clamp(-448.0, 448.0)
+    step = torch.exp2(torch.floor(torch.log2(x.abs().clamp(min=2.0 ** -6))) - 3)
+    return torch.round(x / step) * step
+
+
+def _exact_append(s):
+    """each request's blocks one after the other; a scale is the 32-bit number the cache holds"""
+    kind, bs = s["case"]["codes"], s["case"]["block"]
+    half = CODE_MAX[kind]
+    nearest = _nearest_e4m3 if kind == "fp8" else lambda x: torch.round(x.clamp(-128.0, 127.0))
+    slots = s["slots"].tolist()
+    runs, begin = [], 0
+    for t in range(1, len(slots) + 1):
+        if t == len(slots) or slots[t] // bs != slots[begin] // bs:
+            runs.append((begin, t, slots[begin] // bs, slots[begin] % bs))
+            begin = t
+    out = []
+    for x, codes, scale, transposed in ((s["k"], s["cache"][0], s["cache"][2], False),
+                                        (s["v"], s["cache"][1], s["cache"][3], True)):
+        codes, scale = _code_values(codes), scale.double()
+        for begin, end, block, at in runs:
+            rows = x[begin:end].double()
+            fits = (rows.abs().amax(dim=(0, 2)) / half).float().double().clamp(min=EPS)
+            now = fits if at == 0 else torch.maximum(scale[block], fits)
+            new = nearest(rows / now.view(1, -1, 1))
+            view = codes[block].transpose(1, 2) if transposed else codes[block]
+            view[:, :at] = nearest(view[:, :at] * (scale[block] / now).view(-1, 1, 1))
+            view[:, at:at + end - begin] = new.transpose(0, 1)
+            scale[block] = now
+        out += [codes if kind == "fp8" else codes.to(torch.int8), scale]
+    return out
+
+
+def _exact_attend(s):
+    c = s["case"]
+    share, new, d, bs = c["heads"] // c["kv_heads"], c["new"], c["head_dim"], c["block"]
+    key, value, key_scale, value_scale = s["cache"]
+    out = torch.zeros(s["q"].shape, dtype=torch.float64, device="cuda")
+    for r, n in enumerate(s["lens"].tolist()):
+        blocks = s["table"][r, :-(-n // bs)].long()
+        for h in range(c["kv_heads"]):
+            k = _code_values(key[:, h].view(torch.uint8)[blocks].view(key.dtype)) * key_scale[blocks, h].double().view(-1, 1, 1)
+            v = _code_values(value[:, h].view(torch.uint8)[blocks].view(value.dtype)) * value_scale[blocks, h].double().view(-1, 1, 1)
+            k = k.reshape(-1, d)[:n].t().contiguous()
+            v = v.transpose(1, 2).reshape(-1, d)[:n].contiguous()
+            seen = torch.arange(n, device="cuda").view(1, -1) <= torch.arange(n - new, n, device="cuda").view(-1, 1)
+            for i in range(h * share, (h + 1) * share):
+                score = (s["q"][r * new:(r + 1) * new, i].double() @ k) / math.sqrt(d)
+                weight = torch.softmax(torch.where(seen, score, torch.full_like(score, float("-inf"))), dim=-1)
+                out[r * new:(r + 1) * new, i] = weight @ v
+    return out
+
+
+def exact(case, seed):
+    state = prepare(case, seed)
+    if case["op"] == "plan":
+        return None  # whole numbers
+    return {"linear": _exact_linear, "append": _exact_append, "attend": _exact_attend}[case["op"]](state)
