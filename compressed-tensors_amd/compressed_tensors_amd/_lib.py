@@ -168,6 +168,14 @@ class Stacked24Job(ctypes.Structure):
     ]
 
 
+class KVBlocksC(ctypes.Structure):
+    """mirror of `struct ctmi_kv_blocks`"""
+
+    _fields_ = [("key", c_void_p), ("value", c_void_p), ("key_scale", c_void_p), ("value_scale", c_void_p),
+                ("num_blocks", c_int64), ("kv_heads", c_int32), ("head_dim", c_int32),
+                ("block_size", c_int32), ("code_dtype", c_int32)]
+
+
 class QdqJob(ctypes.Structure):
     """ctmi_qdq_job"""
 
@@ -397,6 +405,30 @@ SIGNATURES = {
         [c_void_p, c_int32, c_int64, c_int64, c_int64, c_int32, c_int32, c_int32, c_void_p,
          c_void_p, c_int32, c_void_p, c_int32, c_void_p, c_void_p, c_void_p],
     ),
+    "ctmi_packed_linear_tmp_bytes": (c_int64, [c_int64, c_int64, c_int64, c_int64]),
+    "ctmi_packed_linear": (
+        c_int32,
+        [c_void_p, c_int32, c_int64, c_void_p, c_void_p, c_int32, c_void_p, c_void_p, c_void_p,
+         c_int64, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p],
+    ),
+    "ctmi_kv_append": (
+        c_int32,
+        [c_void_p, c_void_p, c_int32, c_int64, c_int64, c_int64, c_int64, c_void_p, c_int64,
+         POINTER(KVBlocksC), c_int32, c_void_p],
+    ),
+    "ctmi_kv_attend_tmp_bytes": (
+        c_int64, [c_int64, c_int64, c_int32, c_int32, c_int32, c_int64, c_int64]),
+    "ctmi_kv_attend": (
+        c_int32,
+        [c_void_p, c_int32, c_int64, c_int64, c_void_p, c_int64, c_int32, POINTER(KVBlocksC), c_void_p,
+         c_int64, c_int64, c_void_p, c_void_p, c_int64, c_float, c_int64, c_int64, c_void_p, c_int64,
+         c_void_p],
+    ),
+    "ctmi_kv_plan": (
+        c_int32,
+        [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int32,
+         c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
+    ),
 }
 
 _lib: Optional[ctypes.CDLL] = None
@@ -460,6 +492,26 @@ def ptr(t: Optional[torch.Tensor]) -> Optional[int]:
 # torch's own shortcut to the current stream's handle (what its compiled kernels' launchers
 # call): a tenth of the cost of building a torch.cuda.Stream object on every library call
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+class _SameDevice:
+    """a context that changes nothing"""
+
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return None
+
+
+_SAME_DEVICE = _SameDevice()
+
+
+def on_device(device: torch.device):
+    """context in which kernels and allocations go to `device` (free where it is current)"""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _SAME_DEVICE
+    return torch.cuda.device(device)
 
 
 def stream_of(device: torch.device) -> int:

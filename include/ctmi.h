@@ -721,6 +721,100 @@ int ctmi_kron_matmul(const void* x, void* out, int32_t io_dtype, int64_t numel, 
 int ctmi_block_matmul(const void* x, void* out, int32_t io_dtype, int64_t numel, int32_t h,
                       const float* w, void* stream);
 
+/* ---- what a model answers with: products with packed weights, the 8-bit block cache.
+ * No counterpart in the reference, which decompresses a weight before its first product
+ * (linear/compressed_linear.py:96-109) and keeps a fake-quantized cache in 16 bits
+ * (modeling/kvcache.py:41-96); the formats read here are its own: weight_packed,
+ * weight_scale and the packed weight_zero_point of pack_quantized.py:52-183, and the 8-bit
+ * codes and scales of calculate_qparams (quantization/utils/helpers.py:67-146).
+ *
+ * out[m, n] = round(sum_k x[m, k] * (code[n, k] - zero[n, k / group]) * scale[n, k / group]
+ *                   + bias[n])
+ * for 4-bit codes, the whole sum in fp32 and one rounding to x_dtype.  x [m, k] rows
+ * x_stride elements apart (x_dtype bf16 or f16); packed int32 [n, ceil(k / 8)]; scale
+ * [n, k / group] (f32, f16 or bf16); zero_point NULL or int32 [ceil(n / 8), k / group]
+ * (packed along the rows); bias NULL or x_dtype [n]; out [m, n] contiguous.  group divides
+ * k and is a multiple of 32, or equals k (one scale per row, any k).  tmp: at least
+ * ctmi_packed_linear_tmp_bytes bytes, 16-byte aligned, uninitialised. */
+int64_t ctmi_packed_linear_tmp_bytes(int64_t m, int64_t n, int64_t k, int64_t group);
+int ctmi_packed_linear(const void* x, int32_t x_dtype, int64_t x_stride, const int32_t* packed,
+                       const void* scale, int32_t scale_dtype, const int32_t* zero_point,
+                       const void* bias, void* out, int64_t m, int64_t n, int64_t k, int64_t group,
+                       void* tmp, int64_t tmp_bytes, void* stream);
+
+/* A pool of blocks of block_size tokens (a multiple of 16, 16 ... 256) holding keys and
+ * values as 8-bit codes (CTMI_F8E4M3 or CTMI_I8), one scale per block and head:
+ *   key [num_blocks, kv_heads, block_size, head_dim]
+ *   value [num_blocks, kv_heads, head_dim, block_size]   (tokens innermost)
+ *   key_scale, value_scale fp32 [num_blocks, kv_heads]
+ * key and value 16-byte aligned; head_dim 64, 128 or 256. */
+typedef struct ctmi_kv_blocks {
+  void* key;
+  void* value;
+  float* key_scale;
+  float* value_scale;
+  int64_t num_blocks;
+  int32_t kv_heads, head_dim, block_size, code_dtype;
+} ctmi_kv_blocks;
+
+/* Write new tokens.  key / value: [tokens, kv_heads, head_dim] of `dtype` (bf16 or f16),
+ * strides in elements (head_dim contiguous).  slots: int64 [tokens], block * block_size +
+ * position, tokens of one block next to each other in rising order (what ctmi_kv_plan
+ * writes); a slot outside the pool (-1) skips its token.  A slot named twice in one call is
+ * the caller's mistake: the block it names then holds either token's codes.
+ * dynamic != 0: with A = max|x| over the finite new values of a block and head, the scale
+ * becomes max(A / q, eps), or the maximum of that and the scale it had unless the block's
+ * first position is among the new ones; q = 448 (e4m3) or 127.5 (int8), eps = 2^-23.  Codes
+ * of the positions before the new ones become round(code * (old scale / new scale)).
+ * dynamic == 0: the scales are the caller's and stay.  New codes are x / scale, clamped to
+ * +-448 or [-128, 127] and rounded to nearest even; NaN becomes NaN (e4m3) or 0 (int8). */
+int ctmi_kv_append(const void* key, const void* value, int32_t dtype, int64_t key_token_stride,
+                   int64_t key_head_stride, int64_t value_token_stride, int64_t value_head_stride,
+                   const int64_t* slots, int64_t tokens, const ctmi_kv_blocks* blocks,
+                   int32_t dynamic, void* stream);
+
+/* Attention of new tokens over the pool.  Request r's queries are the tokens
+ * query_start[r] ... query_start[r + 1] - 1 (query_start NULL: token r alone); its keys are
+ * the first seq_lens[r] positions of the blocks block_table[r, 0 ...] names (rows
+ * table_stride apart, `width` entries each).  Query i of n stands at position seq_lens[r] -
+ * n + i and sees the keys up to its own position; one that sees none gives zeros.
+ *   out = softmax(q . k * scale) v,  q [tokens, q_heads, head_dim] (bf16 or f16, strides in
+ * elements), out [tokens, q_heads, head_dim] contiguous, of q's type; query head j reads kv
+ * head j / (q_heads / kv_heads).  Tokens outside every request keep what `out` holds; a
+ * block number outside the pool hides its positions.  max_query and max_seq (the longest
+ * request's queries and keys, as far as the caller knows) only choose the launch: any
+ * values give the same softmax.  tmp: ctmi_kv_attend_tmp_bytes bytes, 16-byte aligned. */
+int64_t ctmi_kv_attend_tmp_bytes(int64_t tokens, int64_t requests, int32_t q_heads,
+                                 int32_t kv_heads, int32_t head_dim, int64_t max_query,
+                                 int64_t max_seq);
+int ctmi_kv_attend(const void* q, int32_t dtype, int64_t q_token_stride, int64_t q_head_stride,
+                   void* out, int64_t tokens, int32_t q_heads, const ctmi_kv_blocks* blocks,
+                   const int32_t* block_table, int64_t table_stride, int64_t width,
+                   const int32_t* seq_lens, const int32_t* query_start, int64_t requests,
+                   float scale, int64_t max_query, int64_t max_seq, void* tmp, int64_t tmp_bytes,
+                   void* stream);
+
+/* The bookkeeping of one serving step.  Request r holds seq_lens[r] tokens in the blocks
+ * block_table[r, ...] names and gains new_tokens[r] >= 0, or ends (new_tokens[r] < 0): its
+ * blocks go back.  free_blocks[0 ... num_free) is a stack.  In request order the blocks of
+ * ended requests are pushed (a request's own in table order), then every block a request
+ * newly needs is popped.  Outputs (none may overlap an input):
+ *   seq_lens_out [requests]          the lengths afterwards (0 for an ended request)
+ *   query_start [requests + 1]       running sum of the new tokens
+ *   slots [slot_count] int64         where each new token goes (ctmi_kv_append), -1 behind
+ *   table_out [requests, width]      with the new blocks; -1 in the rows of ended requests
+ *   free_out [free_capacity], num_free_out [1]   the stack afterwards, -1 behind
+ *   status [1]: 0, or the step did not fit and every output equals its input, slots -1 and
+ *     query_start 0: > 0 that many blocks are missing; -1 a request does not fit its table
+ *     row (or has a negative length); -2 more than slot_count new tokens; -3 the free list
+ *     does not hold what it should (num_free outside 0 ... free_capacity, or more blocks
+ *     come back than fit). */
+int ctmi_kv_plan(const int32_t* seq_lens, const int32_t* new_tokens, const int32_t* block_table,
+                 const int32_t* free_blocks, const int32_t* num_free, int64_t requests,
+                 int64_t width, int64_t free_capacity, int64_t slot_count, int32_t block_size,
+                 int32_t* seq_lens_out, int32_t* query_start, int64_t* slots, int32_t* table_out,
+                 int32_t* free_out, int32_t* num_free_out, int32_t* status, void* stream);
+
 /* Diagnostics, not part of the path: a plain device-to-device copy of `bytes` bytes (a
  * multiple of 16), the known quantity against which hardware byte counters are calibrated
  * when profiling (bench.py --calib-copies).  Nothing in the library or its host mirror
