@@ -5,7 +5,8 @@ Tolerance of the attention.  A score's fp32 sum is off by at most (dim / 32 + 40
 reach = sum |q||k| scale (32 additions inside an instruction, one per instruction, the scales),
 its weight p = exp(score - top) by that (twice: its own and the top's share in the sum) and
 2^-20 for the exponential and the argument's rounding; weights enter the second product as a
-sum of two bf16 numbers (off by 2^-16 of themselves) or, for bf16 outputs, one (2^-9); sums
+sum of two bf16 numbers (off by 2^-16 of themselves) or, for bf16 outputs, one (eps / 2 =
+2^-8: bf16 has 8 significant bits, its neighbours in [1, 2) are 2^-7 apart); sums
 over n keys pass n / 32 + 96 additions.  All of it scales with sum p |v|, and the output's
 rounding is eps / 2 of the value.
 """
@@ -42,7 +43,7 @@ def tables(lens, size, seed=0, spare=2, width=None):
 def check_attention(got, q, blocks, table, lens, starts, scale=None, out=None):
     want, mag, reach = osv.kv_attend(q, blocks, table, lens, starts, scale, out)
     eps, n = torch.finfo(got.dtype).eps, max(int(max(lens)) if len(lens) else 0, 1)
-    weight = 2.0 ** -9 if got.dtype is torch.bfloat16 else 2.0 ** -16
+    weight = 2.0 ** -8 if got.dtype is torch.bfloat16 else 2.0 ** -16
     rel = weight + 2.0 ** -20 + 2 * (q.shape[2] / 32 + 40) * 2.0 ** -24 * reach + (n / 32 + 96) * 2.0 ** -24
     bound = eps / 2 * want.abs() + rel * mag + torch.finfo(got.dtype).smallest_normal * eps
     off = (got.cpu().double() - want).abs()
