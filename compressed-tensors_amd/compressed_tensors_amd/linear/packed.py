@@ -64,11 +64,9 @@ def packed_linear(x: Tensor, weight_packed: Tensor, weight_scale: Tensor,
     device = _lib.require_gpu(x, weight_packed, weight_scale, weight_zero_point, bias)
     weight_packed, weight_scale = weight_packed.contiguous(), weight_scale.contiguous()
     rows = x if x.ndim == 2 else x.reshape(-1, k)
-    # rows of whole 16-byte pieces can be loaded in place
-    if rows.stride(1) != 1 or rows.stride(0) % 8 or rows.data_ptr() % 16 or (rows.shape[0] > 1 and rows.stride(0) < k):
-        rows = rows.contiguous()
-        if rows.data_ptr() % 16:
-            rows = rows.clone(memory_format=torch.contiguous_format)
+    # rows that start at 16-byte boundaries are read in place
+    if rows.stride(1) != 1 or rows.stride(0) % 8 or rows.data_ptr() % 16 or (rows.stride(0) < k and rows.shape[0] > 1):
+        rows = torch.empty((rows.shape[0], (k + 7) // 8 * 8), dtype=x.dtype, device=device)[:, :k].copy_(rows)
     m = rows.shape[0]
     lib = _lib.load()
     with _lib.on_device(device):
