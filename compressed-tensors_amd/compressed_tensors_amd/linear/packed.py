@@ -62,10 +62,13 @@ def packed_linear(x: Tensor, weight_packed: Tensor, weight_scale: Tensor,
             raise ValueError(f"expected a bias {x.dtype} [{n}], got {bias.dtype} {tuple(bias.shape)}")
         bias = bias.contiguous()
     device = _lib.require_gpu(x, weight_packed, weight_scale, weight_zero_point, bias)
+    if weight_scale.dtype is not x.dtype and weight_scale.dtype is not torch.float32:
+        weight_scale = weight_scale.float()
     weight_packed, weight_scale = weight_packed.contiguous(), weight_scale.contiguous()
     rows = x if x.ndim == 2 else x.reshape(-1, k)
     # rows that start at 16-byte boundaries are read in place
-    if rows.stride(1) != 1 or rows.stride(0) % 8 or rows.data_ptr() % 16 or (rows.stride(0) < k and rows.shape[0] > 1):
+    if (rows.stride(1) != 1 or rows.stride(0) % 8 or rows.data_ptr() % 16
+            or (rows.shape[0] > 1 and not k <= rows.stride(0) < 1 << 24)):
         rows = torch.empty((rows.shape[0], (k + 7) // 8 * 8), dtype=x.dtype, device=device)[:, :k].copy_(rows)
     m = rows.shape[0]
     lib = _lib.load()

@@ -42,7 +42,8 @@ struct LinearArgs {
   uint16_t* out;
   float* part;  // [split][m][n], or NULL
   int32_t m, n, k, group, groups, words;
-  int32_t scale_dtype, wave_k;  // columns a wavefront takes
+  int32_t wave_k;  // columns a wavefront takes
+  int32_t pair_groups, pair_rest;  // 256 columns = pair_groups groups and pair_rest columns
 };
 
 struct Operand {
@@ -57,21 +58,22 @@ __device__ __forceinline__ f32x4 product(const Operand& a, const Operand& b, f32
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-// the codes of a word as operands, in the order 0 2 4 6 1 3 5 7
+// the codes of a word as operands: nibbles to bytes in their order, two bytes to two numbers
 template <typename T>
 __device__ __forceinline__ Operand codes_of(uint32_t w) {
   const uint32_t even = w & 0x0F0F0F0Fu, odd = (w >> 4) & 0x0F0F0F0Fu;
+  const uint32_t lo = __builtin_amdgcn_perm(odd, even, 0x05010400u), hi = __builtin_amdgcn_perm(odd, even, 0x07030602u);
   Operand o;
   if constexpr (T::id == CTMI_BF16) {
-    o.w[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(even, 512.0f, false));
-    o.w[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(even, 512.0f, true));
-    o.w[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(odd, 512.0f, false));
-    o.w[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(odd, 512.0f, true));
+    o.w[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 512.0f, false));
+    o.w[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 512.0f, true));
+    o.w[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 512.0f, false));
+    o.w[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 512.0f, true));
   } else {
-    o.w[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(even, 512.0f, false));
-    o.w[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(even, 512.0f, true));
-    o.w[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(odd, 512.0f, false));
-    o.w[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(odd, 512.0f, true));
+    o.w[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 512.0f, false));
+    o.w[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 512.0f, true));
+    o.w[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 512.0f, false));
+    o.w[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 512.0f, true));
   }
   return o;
 }
@@ -82,17 +84,10 @@ __device__ __forceinline__ Operand signed_codes_of(uint32_t w, float zero) {
   Operand o;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    const int at = (e % 2) * 16 + (e / 2) * 4;  // 0 2, 4 6, 1 3, 5 7
-    const float a = (float)((w >> at) & 15) - zero, b = (float)((w >> (at + 8)) & 15) - zero;
+    const float a = (float)((w >> (8 * e)) & 15) - zero, b = (float)((w >> (8 * e + 4)) & 15) - zero;
     o.w[e] = (uint32_t)T::from_f32(a) | ((uint32_t)T::from_f32(b) << 16);
   }
   return o;
-}
-
-// 8 neighbouring elements of x in that order
-__device__ __forceinline__ Operand reorder(const Vec<uint32_t, 4>& x) {
-  return Operand{{__builtin_amdgcn_perm(x.v[1], x.v[0], 0x05040100u), __builtin_amdgcn_perm(x.v[3], x.v[2], 0x05040100u),
-                  __builtin_amdgcn_perm(x.v[1], x.v[0], 0x07060302u), __builtin_amdgcn_perm(x.v[3], x.v[2], 0x07060302u)}};
 }
 
 // The four lane groups hold words 4 j + t; afterwards w[t] is word 4 t + j: 32 neighbouring
@@ -111,173 +106,260 @@ __device__ __forceinline__ void transpose4(uint32_t* w) {
   }
 }
 
+// Loads through a buffer descriptor: an offset behind its end (kNowhere) reads nothing and
+// gives 0, so a wavefront can "load" a step that does not exist without a branch.
+constexpr uint32_t kNowhere = 0x80000000u;
+struct Buffer {
+  __amdgpu_buffer_rsrc_t r;
+  __device__ __forceinline__ Buffer(const void* base, uint32_t bytes)
+      : r(__builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)bytes, 0x00027000)) {}
+  __device__ __forceinline__ Vec<uint32_t, 4> load16(uint32_t at) const {
+    return __builtin_bit_cast(Vec<uint32_t, 4>, __builtin_amdgcn_raw_buffer_load_b128(r, (int)at, 0, 0));
+  }
+  __device__ __forceinline__ uint32_t load4(uint32_t at) const { return __builtin_amdgcn_raw_buffer_load_b32(r, (int)at, 0, 0); }
+  __device__ __forceinline__ uint32_t load2(uint32_t at) const { return __builtin_amdgcn_raw_buffer_load_b16(r, (int)at, 0, 0); }
+};
+
 // SMALL: groups that are no multiple of 128 columns, so a scale holds for one product of 32
-// columns only.  PF steps are requested before the ones in hand are multiplied.
-template <typename T, int MT, int NT, bool SMALL>
+// columns only.  WIDE: scales are fp32, else of x's type.
+//
+// A wavefront keeps two steps requested: a slot is loaded again as soon as its step is
+// multiplied.  The slots are registers by name, the loads stand in no branch (behind the last
+// step they read nothing) and rows behind the last are read as the last (their sums are
+// dropped): a load that may not have been issued, or a copy of a register that is still to
+// arrive, would make the wait for one step a wait for all.  The loop holds the two steps and
+// nothing is unrolled beyond them: a wavefront runs few steps, and code it has to fetch for
+// each of them costs more than the steps do.
+template <typename T, int MT, int NT, bool SMALL, bool WIDE>
 struct LinearWave {
-  static constexpr int PF = SMALL ? (NT == 1 ? 2 : 1) : (NT == 1 ? 4 : NT == 2 ? 2 : 1);
-  static constexpr int SC = SMALL ? 4 : 1;  // scales per step
-
-  const LinearArgs& a;
-  int lane, c, j, m0;
-  int row[NT];  // weight row of each tile, within the weight
-  f32x4 y[NT][MT];
-
   struct Step {
-    uint32_t w[NT][4];
-    float s[NT][SC], z[NT][SC];
+    Vec<uint32_t, 4> w[NT];
+    Vec<uint32_t, 4> x[MT][4];
+  };
+  // as loaded, for a pair of steps, a different group in each lane group.  SMALL: entry i is
+  // step i, lane group j its columns 32 j ... 32 j + 31; otherwise lane group j is step j % 2.
+  static constexpr int RAW = SMALL ? 2 : 1;
+  struct Scales {
+    uint32_t s[RAW][NT], z[RAW][NT];
   };
 
-  __device__ __forceinline__ void load(Step& st, int kb) {
-    const bool whole = kb + kStepK <= a.k && a.words % 4 == 0;
+  const LinearArgs& a;
+  int c, j;
+  // where there are no zero points the buffer is empty, reads 0, and every zero point is 8
+  uint32_t z_none;
+  Buffer w_buf, s_buf, z_buf, x_buf;  // of the workgroup's rows
+  uint32_t w_at[NT], s_at[NT], z_at[NT], x_at[MT];
+  f32x4 y[NT][MT];
+
+  __device__ __forceinline__ LinearWave(const LinearArgs& args, int n0, int m0)
+      : a(args),
+        w_buf(a.packed + (int64_t)n0 * a.words, (uint32_t)min(NT * 16, a.n - n0) * (uint32_t)a.words * 4u),
+        s_buf((const uint8_t*)a.scale + (int64_t)n0 * a.groups * (WIDE ? 4 : 2),
+              (uint32_t)min(NT * 16, a.n - n0) * (uint32_t)a.groups * (WIDE ? 4 : 2)),
+        z_buf(a.zero + (int64_t)(n0 >> 3) * a.groups, a.zero ? (uint32_t)((min(NT * 16, a.n - n0) + 7) >> 3) * (uint32_t)a.groups * 4u : 0u),
+        x_buf(a.x + m0 * a.x_stride, ((uint32_t)(min(MT * 16, a.m - m0) - 1) * (uint32_t)a.x_stride + (uint32_t)a.k) * 2u) {
+    const int lane = lane_id();
+    c = lane & 15, j = lane >> 4;
+    z_none = a.zero ? 0u : 8u;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      const uint32_t* p = a.packed + (int64_t)row[t] * a.words;
-      const int w0 = kb / 8 + j * 4;
-      if (whole && ((uintptr_t)a.packed & 15) == 0) {
-        const Vec<uint32_t, 4> v = ldg_nt<uint32_t, 4>(p + w0);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) st.w[t][i] = v.v[i];
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) st.w[t][i] = w0 + i < a.words ? p[w0 + i] : 0u;
-      }
-#pragma unroll
-      for (int i = 0; i < SC; ++i) {
-        const int g = min((kb + i * 32) / a.group, a.groups - 1);
-        st.s[t][i] = load_f32(a.scale, a.scale_dtype, (int64_t)row[t] * a.groups + g);
-        st.z[t][i] = a.zero ? (float)((a.zero[(int64_t)(row[t] >> 3) * a.groups + g] >> (4 * (row[t] & 7))) & 15u) : 8.0f;
-      }
+      const int row = min(t * 16 + c, a.n - 1 - n0);  // n0 is a multiple of 16
+      w_at[t] = (uint32_t)row * (uint32_t)a.words * 4u + j * 16;
+      s_at[t] = (uint32_t)row * (uint32_t)a.groups * (WIDE ? 4 : 2);
+      z_at[t] = (uint32_t)(row >> 3) * (uint32_t)a.groups * 4u;
     }
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+      x_at[mt] = (uint32_t)min(mt * 16 + c, a.m - 1 - m0) * (uint32_t)a.x_stride * 2u + j * 16;
+    clear();
   }
 
-  template <bool SIGNED>
-  __device__ __forceinline__ void step(Step& st, int kb) {
-    const Operand ones = T::id == CTMI_BF16 ? Operand{{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u}}
-                                            : Operand{{0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u}};
-    Operand x[MT][4];
+  __device__ __forceinline__ void clear() {
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      const int m = m0 + mt * 16 + c;
-      const uint16_t* p = a.x + (int64_t)m * a.x_stride;
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) y[t][mt] = f32x4{0, 0, 0, 0};
+  }
+
+  // the group of this lane's columns in pairs of steps as they are loaded, one after the other
+  struct Groups {
+    int g[RAW], left[RAW];  // and how many columns of it follow
+  };
+  __device__ __forceinline__ Groups groups_at(int kb) const {
+    Groups at;
+#pragma unroll
+    for (int i = 0; i < RAW; ++i) {
+      const int k = kb + (SMALL ? i * kStepK + j * 32 : (j & 1) * kStepK);
+      at.g[i] = k / a.group, at.left[i] = (at.g[i] + 1) * a.group - k;
+    }
+    return at;
+  }
+  __device__ __forceinline__ void load_scales(Scales& sc, Groups& at) const {
+#pragma unroll
+    for (int i = 0; i < RAW; ++i) {
+      const uint32_t g = min(at.g[i], a.groups - 1);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        sc.s[i][t] = WIDE ? s_buf.load4(s_at[t] + g * 4u) : s_buf.load2(s_at[t] + g * 2u);
+        sc.z[i][t] = z_buf.load4(z_at[t] + g * 4u);
+      }
+      at.g[i] += a.pair_groups, at.left[i] -= a.pair_rest;
+      if (at.left[i] <= 0) at.left[i] += a.group, ++at.g[i];
+    }
+  }
+  __device__ __forceinline__ float scale_of(uint32_t raw) const { return WIDE ? u2f(raw) : T::to_f32((uint16_t)raw); }
+  __device__ __forceinline__ float zero_of(uint32_t raw) const { return (float)(((raw >> (4 * (c & 7))) & 15u) | z_none); }
+
+  __device__ __forceinline__ void load(Step& st, int kb, bool there) const {
+    const uint32_t wk = there ? (uint32_t)kb / 2u : kNowhere, xk = there ? (uint32_t)kb * 2u : kNowhere;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) st.w[t] = w_buf.load16(w_at[t] + wk);
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int t = 0; t < 4; ++t) st.x[mt][t] = x_buf.load16(x_at[mt] + xk + t * 64);
+  }
+
+  // a step that may end behind the row, or of rows that do not start at 16-byte boundaries
+  __device__ __forceinline__ void load_guarded(Step& st, int kb) const {
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        st.w[t].v[i] = w_buf.load4(kb / 8 + j * 4 + i < a.words ? w_at[t] + kb / 2 + i * 4 : kNowhere);
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        const int at = kb + (SMALL ? t * 32 + j * 8 : j * 32 + t * 8);
-        Vec<uint32_t, 4> v = {};
-        if (m < a.m) {
-          if (at + 8 <= a.k) {
-            v = ldg<uint32_t, 4>((const uint32_t*)(p + at));
-          } else {
+        const int first = kb + t * 32 + j * 8;
+        const uint32_t at = x_at[mt] + kb * 2 + t * 64;
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (at + e < a.k) v.v[e / 2] |= (uint32_t)p[at + e] << (16 * (e % 2));
-          }
-        }
-        x[mt][t] = reorder(v);
+        for (int e = 0; e < 4; ++e)
+          st.x[mt][t].v[e] = x_buf.load2(first + 2 * e < a.k ? at + 4 * e : kNowhere) |
+                             x_buf.load2(first + 2 * e + 1 < a.k ? at + 4 * e + 2 : kNowhere) << 16;
       }
-    }
-    f32x4 sums[MT];
-    if constexpr (!SIGNED && !SMALL) {
+  }
+
+  // s, z: scale and zero point of each tile's column and, SMALL, of this lane's 32 columns
+  template <bool SIGNED>
+  __device__ __forceinline__ void step(Step& st, const float* scales, const float* zeros) {
+    const Operand ones = T::id == CTMI_BF16 ? Operand{{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u}}
+                                            : Operand{{0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u}};
+    constexpr int PARTS = SMALL ? 4 : 1;
+    f32x4 sums[PARTS][MT];
+    if constexpr (!SIGNED) {
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
-        sums[mt] = f32x4{0, 0, 0, 0};
 #pragma unroll
-        for (int t = 0; t < 4; ++t) sums[mt] = product<T>(x[mt][t], ones, sums[mt]);
+        for (int i = 0; i < PARTS; ++i) sums[i][mt] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+          sums[SMALL ? t : 0][mt] = product<T>(__builtin_bit_cast(Operand, st.x[mt][t]), ones, sums[SMALL ? t : 0][mt]);
       }
     }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      if constexpr (SMALL) transpose4(st.w[nt]);
+      transpose4(st.w[nt].v);
+      float s = scales[nt], z = zeros[nt];
       f32x4 acc[MT];
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) acc[mt] = f32x4{0, 0, 0, 0};
-#pragma unroll
       for (int t = 0; t < 4; ++t) {
-        const int at = SMALL ? t : 0;
-        Operand w;
-        if constexpr (SIGNED) w = signed_codes_of<T>(st.w[nt][t], st.z[nt][at]);
-        else w = codes_of<T>(st.w[nt][t]);
+        if constexpr (SMALL) s = __shfl(scales[nt], t * 16 + c, kWave), z = __shfl(zeros[nt], t * 16 + c, kWave);
+        const Operand w = SIGNED ? signed_codes_of<T>(st.w[nt].v[t], z) : codes_of<T>(st.w[nt].v[t]);
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
-          acc[mt] = product<T>(x[mt][t], w, acc[mt]);
-          if constexpr (SMALL) {
-            if constexpr (!SIGNED) sums[mt] = product<T>(x[mt][t], ones, f32x4{0, 0, 0, 0});
+          if (t == 0 || SMALL) acc[mt] = f32x4{0, 0, 0, 0};
+          acc[mt] = product<T>(__builtin_bit_cast(Operand, st.x[mt][t]), w, acc[mt]);
+          if (SMALL || t == 3) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const float v = SIGNED ? acc[mt][i] : fmaf(-st.z[nt][at], sums[mt][i], acc[mt][i]);
-              y[nt][mt][i] = fmaf(st.s[nt][at], v, y[nt][mt][i]);
+              const float v = SIGNED ? acc[mt][i] : fmaf(-z, sums[SMALL ? t : 0][mt][i], acc[mt][i]);
+              y[nt][mt][i] = fmaf(s, v, y[nt][mt][i]);
             }
-            acc[mt] = f32x4{0, 0, 0, 0};
           }
         }
-      }
-      if constexpr (!SMALL) {
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float v = SIGNED ? acc[mt][i] : fmaf(-st.z[nt][0], sums[mt][i], acc[mt][i]);
-            y[nt][mt][i] = fmaf(st.s[nt][0], v, y[nt][mt][i]);
-          }
       }
     }
   }
 
-  template <bool SIGNED>
-  __device__ __forceinline__ void run(int k0, int k1) {
+  // the scales of a pair's steps, in the lanes that use them
+  __device__ __forceinline__ void spread(const Scales& raw, float (*s)[NT], float (*z)[NT]) const {
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) y[nt][mt] = f32x4{0, 0, 0, 0};
-    Step now[PF];
-#pragma unroll
-    for (int p = 0; p < PF; ++p)
-      if (k0 + p * kStepK < k1) load(now[p], k0 + p * kStepK);
-    for (int kb = k0; kb < k1; kb += PF * kStepK) {
-      Step next[PF];
-#pragma unroll
-      for (int p = 0; p < PF; ++p) {
-        const int at = kb + (PF + p) * kStepK;
-        if (at < k1) load(next[p], at);
+      for (int t = 0; t < NT; ++t) {
+        if constexpr (SMALL) {
+          s[i][t] = scale_of(raw.s[i][t]), z[i][t] = zero_of(raw.z[i][t]);
+        } else {
+          s[i][t] = __shfl(scale_of(raw.s[0][t]), i * 16 + c, kWave);
+          z[i][t] = __shfl(zero_of(raw.z[0][t]), i * 16 + c, kWave);
+        }
       }
-#pragma unroll
-      for (int p = 0; p < PF; ++p)
-        if (kb + p * kStepK < k1) step<SIGNED>(now[p], kb + p * kStepK);
-#pragma unroll
-      for (int p = 0; p < PF; ++p) now[p] = next[p];
+  }
+
+  // columns k0 ... k1 - 1; those behind the last whole step (all of them, if the rows of the
+  // weight do not start at 16-byte boundaries) are left to run_signed
+  __device__ __forceinline__ int run(int k0, int k1) {
+    const bool aligned = a.words % 4 == 0 && ((uintptr_t)a.packed & 15) == 0;
+    const int end = aligned ? k0 + (min(k1, a.k) - k0) / kStepK * kStepK : k0;
+    if (k0 < end) {
+      Step one, two;
+      Scales raw;
+      Groups at = groups_at(k0);
+      load_scales(raw, at);
+      load(one, k0, true);
+      load(two, k0 + kStepK, k0 + kStepK < end);
+#pragma unroll 1
+      for (int kb = k0; kb < end; kb += 2 * kStepK) {
+        float s[2][NT], z[2][NT];
+        spread(raw, s, z);
+        load_scales(raw, at);
+        step<false>(one, s[0], z[0]);
+        load(one, kb + 2 * kStepK, kb + 2 * kStepK < end);
+        __builtin_amdgcn_sched_barrier(0);
+        step<false>(two, s[1], z[1]);
+        load(two, kb + 3 * kStepK, kb + 3 * kStepK < end);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    return end;
+  }
+
+  __device__ __forceinline__ void run_signed(int k0, int k1) {
+#pragma unroll 1
+    for (int kb = k0; kb < k1; kb += kStepK) {
+      Step st;
+      Scales raw;
+      Groups at = groups_at(kb);
+      float s[2][NT], z[2][NT];
+      load_guarded(st, kb);
+      load_scales(raw, at);
+      spread(raw, s, z);
+      step<true>(st, s[0], z[0]);
     }
   }
 };
 
-template <typename T, int MT, int NT, bool SMALL, int WAVES>
-__global__ __launch_bounds__(WAVES* kWave) void packed_linear_kernel(LinearArgs a) {
+template <typename T, int MT, int NT, bool SMALL, bool WIDE, int WAVES, int PER_SIMD>
+__global__ __launch_bounds__(WAVES* kWave, PER_SIMD) void packed_linear_kernel(LinearArgs a) {
   constexpr int TM = MT * 16, TN = NT * 16;
   extern __shared__ float meet[];  // [wave][TM][TN]
   const int wave = threadIdx.x / kWave, waves = blockDim.x / kWave;
   const int n0 = blockIdx.x * TN;
-  LinearWave<T, MT, NT, SMALL> w{a};
-  w.lane = lane_id(), w.c = w.lane & 15, w.j = w.lane >> 4, w.m0 = blockIdx.y * TM;
+  LinearWave<T, MT, NT, SMALL, WIDE> w(a, n0, blockIdx.y * TM);
+  const int64_t begin = ((int64_t)blockIdx.z * waves + wave) * a.wave_k;
+  const int k0 = (int)(begin < a.k ? begin : a.k), k1 = (int)(begin + a.wave_k < a.k ? begin + a.wave_k : a.k);
+  int redo = w.run((int)k0, k1);
+  bool bad = false;
 #pragma unroll
-  for (int t = 0; t < NT; ++t) w.row[t] = min(n0 + t * 16 + w.c, a.n - 1);
-  const int64_t k0 = ((int64_t)blockIdx.z * waves + wave) * a.wave_k;
-  const int k1 = (int)(k0 + a.wave_k < a.k ? k0 + a.wave_k : a.k);
-  if (k0 < k1) {
-    w.template run<false>((int)k0, k1);
-    bool bad = false;
+  for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) bad |= !(fabsf(w.y[nt][mt][i]) <= 3.4028235e38f);
-    if (__any(bad)) w.template run<true>((int)k0, k1);
-  } else {
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) w.y[nt][mt] = f32x4{0, 0, 0, 0};
-  }
-  const int rows = min(TM, a.m - w.m0);
+      for (int i = 0; i < 4; ++i) bad |= !(fabsf(w.y[nt][mt][i]) <= 3.4028235e38f);
+  if (__any(bad)) w.clear(), redo = (int)k0;
+  w.run_signed(redo, k1);
+  const int m0 = blockIdx.y * TM, rows = min(TM, a.m - m0);
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -293,7 +375,7 @@ __global__ __launch_bounds__(WAVES* kWave) void packed_linear_kernel(LinearArgs 
     float v = 0.0f;
     for (int i = 0; i < waves; ++i) v += meet[i * TM * TN + at];
     if (n < a.n) {
-      const int64_t cell = (int64_t)(w.m0 + r) * a.n + n;
+      const int64_t cell = (int64_t)(m0 + r) * a.n + n;
       if (a.part) a.part[(int64_t)blockIdx.z * a.m * a.n + cell] = v;
       else a.out[cell] = T::from_f32(v + (a.bias ? T::to_f32(a.bias[n]) : 0.0f));
     }
@@ -322,12 +404,11 @@ LinearLaunch plan_linear(int64_t m, int64_t n, int64_t k) {
   l.splits = 1;
   if (l.mt == 1) {
     l.nt = tiles >= 1024 ? 4 : tiles >= 512 ? 2 : 1;
-    l.waves = 8;
-    if (k > 8 * 512 && tiles <= 512) l.waves = 16;
+    l.waves = l.nt == 4 ? 4 : 8;
   } else {
-    l.nt = 4;
+    l.nt = l.mt == 4 ? 2 : 4;
     l.waves = 4;
-    const int64_t units = cdiv(n, 64) * m_blocks;
+    const int64_t units = cdiv(tiles, l.nt) * m_blocks;
     while (units * l.splits < 256 && k / (l.waves * l.splits * 2) >= 256 && l.splits < 16) l.splits *= 2;
   }
   l.wave_k = cdiv(cdiv(k, l.waves * l.splits), kStepK) * kStepK;
@@ -351,12 +432,12 @@ extern "C" int ctmi_packed_linear(const void* x, int32_t x_dtype, int64_t x_stri
                                   int64_t group, void* tmp, int64_t tmp_bytes, void* stream) {
   CTMI_REQUIRE(x_dtype == CTMI_BF16 || x_dtype == CTMI_F16, CTMI_ERR_UNSUPPORTED,
                "activations must be bfloat16 or float16");
-  CTMI_REQUIRE(scale_dtype == CTMI_F32 || scale_dtype == CTMI_F16 || scale_dtype == CTMI_BF16,
-               CTMI_ERR_UNSUPPORTED, "unsupported scale dtype %d", scale_dtype);
+  CTMI_REQUIRE(scale_dtype == CTMI_F32 || scale_dtype == x_dtype, CTMI_ERR_UNSUPPORTED,
+               "scales must be float32 or of x's type, got dtype %d", scale_dtype);
   CTMI_REQUIRE(m >= 0 && n >= 0 && k >= 1, CTMI_ERR_VALUE, "bad sizes [%lld, %lld] x [%lld, %lld]",
                (long long)m, (long long)k, (long long)n, (long long)k);
-  CTMI_REQUIRE(m < (1ll << 31) && n < (1ll << 31) && k < (1ll << 31), CTMI_ERR_UNSUPPORTED,
-               "sizes must stay below 2^31");
+  CTMI_REQUIRE(m < (1ll << 31) && n < (1ll << 31) && k <= (1ll << 24), CTMI_ERR_UNSUPPORTED,
+               "sizes must stay below 2^31 (columns: 2^24)");
   CTMI_REQUIRE(group == k || (group >= 32 && group % 32 == 0 && k % group == 0), CTMI_ERR_UNSUPPORTED,
                "groups of %lld do not fit %lld columns: a multiple of 32 that divides them, or one group",
                (long long)group, (long long)k);
@@ -366,6 +447,7 @@ extern "C" int ctmi_packed_linear(const void* x, int32_t x_dtype, int64_t x_stri
   CTMI_REQUIRE(x && packed && scale && out, CTMI_ERR_VALUE, "NULL tensor");
   CTMI_REQUIRE(((uintptr_t)x % 16 == 0) && (x_stride % 8 == 0 || m == 1), CTMI_ERR_VALUE,
                "rows of x must start at 16-byte boundaries");
+  CTMI_REQUIRE(x_stride < (1ll << 24) || m == 1, CTMI_ERR_UNSUPPORTED, "rows of x more than 2^24 elements apart");
   const LinearLaunch l = plan_linear(m, n, k);
   const int64_t need = l.splits > 1 ? l.splits * m * n * 4 : 0;
   CTMI_REQUIRE(tmp_bytes >= need && (need == 0 || (tmp != nullptr && (uintptr_t)tmp % 16 == 0)), CTMI_ERR_VALUE,
@@ -374,21 +456,29 @@ extern "C" int ctmi_packed_linear(const void* x, int32_t x_dtype, int64_t x_stri
   CTMI_REQUIRE(cdiv(m, tm) < (1 << 16), CTMI_ERR_UNSUPPORTED, "too many rows: %lld", (long long)m);
   LinearArgs a{(const uint16_t*)x, x_stride, (const uint32_t*)packed, scale, (const uint32_t*)zero_point,
                (const uint16_t*)bias, (uint16_t*)out, need ? (float*)tmp : nullptr, (int32_t)m, (int32_t)n,
-               (int32_t)k, (int32_t)group, (int32_t)(k / group), (int32_t)cdiv(k, 8), scale_dtype,
-               (int32_t)l.wave_k};
+               (int32_t)k, (int32_t)group, (int32_t)(k / group), (int32_t)cdiv(k, 8), (int32_t)l.wave_k,
+               (int32_t)(2 * kStepK / group), (int32_t)(2 * kStepK % group)};
   const dim3 grid((unsigned)cdiv(n, tn), (unsigned)cdiv(m, tm), (unsigned)l.splits), threads(l.waves * kWave);
   const size_t lds = (size_t)l.waves * tm * tn * sizeof(float);
   const hipStream_t s = (hipStream_t)stream;
   const bool small = group % kStepK != 0 && group != k;
-#define LAUNCH(T, MT, NT, W) do { if (small) packed_linear_kernel<T, MT, NT, true, W><<<grid, threads, lds, s>>>(a); \
-                                  else packed_linear_kernel<T, MT, NT, false, W><<<grid, threads, lds, s>>>(a); } while (0)
+#define LAUNCH(T, MT, NT, W, P)                                                                       \
+  do {                                                                                                \
+    if (scale_dtype == CTMI_F32) {                                                                    \
+      if (small) packed_linear_kernel<T, MT, NT, true, true, W, P><<<grid, threads, lds, s>>>(a);     \
+      else packed_linear_kernel<T, MT, NT, false, true, W, P><<<grid, threads, lds, s>>>(a);          \
+    } else {                                                                                          \
+      if (small) packed_linear_kernel<T, MT, NT, true, false, W, P><<<grid, threads, lds, s>>>(a);    \
+      else packed_linear_kernel<T, MT, NT, false, false, W, P><<<grid, threads, lds, s>>>(a);         \
+    }                                                                                                 \
+  } while (0)
 #define BY_SIZE(T)                                  \
   do {                                              \
-    if (l.mt == 4) LAUNCH(T, 4, 4, 4);              \
-    else if (l.mt == 2) LAUNCH(T, 2, 4, 4);         \
-    else if (l.nt == 4) LAUNCH(T, 1, 4, 8);         \
-    else if (l.nt == 2) LAUNCH(T, 1, 2, 16);        \
-    else LAUNCH(T, 1, 1, 16);                       \
+    if (l.mt == 4) LAUNCH(T, 4, 2, 4, 2);           \
+    else if (l.mt == 2) LAUNCH(T, 2, 4, 4, 2);      \
+    else if (l.nt == 4) LAUNCH(T, 1, 4, 4, 3);      \
+    else if (l.nt == 2) LAUNCH(T, 1, 2, 8, 4);      \
+    else LAUNCH(T, 1, 1, 8, 4);                     \
     if (need) packed_linear_join_kernel<T><<<dim3((unsigned)(cdiv(m * n, 256) < 2048 ? cdiv(m * n, 256) : 2048)), dim3(256), 0, s>>>(a, (int)l.splits); \
   } while (0)
   if (x_dtype == CTMI_BF16) BY_SIZE(BF16);

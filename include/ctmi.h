@@ -732,7 +732,7 @@ int ctmi_block_matmul(const void* x, void* out, int32_t io_dtype, int64_t numel,
  *                   + bias[n])
  * for 4-bit codes, the whole sum in fp32 and one rounding to x_dtype.  x [m, k] rows
  * x_stride elements apart (x_dtype bf16 or f16); packed int32 [n, ceil(k / 8)]; scale
- * [n, k / group] (f32, f16 or bf16); zero_point NULL or int32 [ceil(n / 8), k / group]
+ * [n, k / group] (f32 or x_dtype); zero_point NULL or int32 [ceil(n / 8), k / group]
  * (packed along the rows); bias NULL or x_dtype [n]; out [m, n] contiguous.  group divides
  * k and is a multiple of 32, or equals k (one scale per row, any k).  tmp: at least
  * ctmi_packed_linear_tmp_bytes bytes, 16-byte aligned, uninitialised. */

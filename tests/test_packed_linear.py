@@ -52,7 +52,8 @@ SHAPES = [  # m, n, k, groups
 def test_shapes(gpu, m, n, k, groups, dtype):
     from compressed_tensors_amd.linear import packed_linear
 
-    for asym, bias, scale_dtype in ((False, False, None), (True, True, None), (True, False, torch.float32)):
+    for asym, bias, scale_dtype in ((False, False, None), (True, True, None), (True, False, torch.float32),
+                                    (False, True, torch.float16 if dtype is torch.bfloat16 else torch.bfloat16)):
         announce("packed_linear", m, n, k, groups, dtype, asym, bias, scale_dtype)
         data = make(m, n, k, groups, dtype, scale_dtype, asym, bias, seed=m + n + k)
         check(packed_linear(*on(gpu, *data)), *data)
