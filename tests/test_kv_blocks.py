@@ -503,14 +503,14 @@ def test_abi_refusals(ctmi):
     def blocks(num=4, heads=2, dim=64, size=16, code=3, at=16):
         return KVBlocksC(at, at, at, at, num, heads, dim, size, code)
 
-    def append(b, dtype=2, tokens=2, at=16):
-        return ctmi.ctmi_kv_append(at, at, dtype, 128, 64, 128, 64, at, tokens, byref(b), 1, None)
+    def append(b, dtype=2, tokens=2, at=16, stride=128):
+        return ctmi.ctmi_kv_append(at, at, dtype, stride, 64, 128, 64, at, tokens, byref(b), 1, None)
 
     for bad, code in ((blocks(dim=80), -2), (blocks(size=24), -2), (blocks(size=272), -2), (blocks(code=8), -2),
                       (blocks(heads=0), -1), (blocks(num=-1), -1), (blocks(at=0), -1), (blocks(at=8), -1)):
         assert append(bad) == code
     assert append(blocks(), dtype=0) == -2 and append(blocks(), tokens=-1) == -1 and append(blocks(), at=0) == -1
-    assert append(blocks(), tokens=0) == 0
+    assert append(blocks(), tokens=0) == 0 and append(blocks(), stride=100) == -1 and append(blocks(), at=24) == -1
 
     def attend(b=None, dtype=2, tokens=2, heads=4, stride=128, width=3, table_stride=3, requests=2, start=16, at=16,
                max_query=1, max_seq=48, tmp=0):
