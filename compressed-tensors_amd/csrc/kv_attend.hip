@@ -16,13 +16,13 @@
 // the second product wants keys in groups j, too.  Taking key (r / 4) * 16 + t * 4 + r % 4 as
 // row r of key tile t gives group j the 16 neighbouring keys 16 j ... 16 j + 15: P needs no
 // exchange, and with tokens innermost in the value blocks a lane's V operand is one 16-byte
-// load.  No LDS in the loop; keys and values go from memory into operand registers, the next
-// step's keys are requested when this step's are used up, and so are the values.
+// load.  The next step's keys are requested when this step's are used up, and so are the
+// values.
 //
-// KS: the four wavefronts of a workgroup share the rows and split the keys (few rows: a
-// decode step) and meet in LDS at the end; otherwise they take rows of their own.  A long
-// axis is cut into chunks for several workgroups, whose unnormalised sums, maxima and
-// weights meet in a second, small kernel.
+// With few rows (a decode step) the four wavefronts of a workgroup share them, split the keys
+// and meet in LDS at the end; with many they take rows of their own and share the keys through
+// LDS.  A long axis is cut into chunks for several workgroups, whose unnormalised sums, maxima
+// and weights meet in a second, small kernel.
 #include "kv_blocks.h"
 
 namespace ctmi {
@@ -144,38 +144,22 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
   return (((w & 0x7F7F7F7Fu) + 0x01010101u) >> 7 & 0x01010101u) * 0xFFu;
 }
 
-template <typename T, bool FP8, int D, int RT, bool KS, bool SPLIT>
-__global__ __launch_bounds__(kAttendWaves* kWave) void kv_attend_kernel(AttendArgs a) {
-  constexpr int CH = D / 64;   // 16-byte pieces of a key per lane
-  constexpr int DT = D / 16;   // tiles of the output's dimensions
-  constexpr int ROWS = (KS ? 1 : kAttendWaves) * RT * 16;  // of a workgroup
-  const int lane = lane_id(), wave = threadIdx.x / kWave, c = lane & 15, j = lane >> 4;
-  const int share = a.q_heads / a.kv_heads;
-  int id = blockIdx.x;
-  const int kv = id % a.kv_heads;
-  id /= a.kv_heads;
-  const int chunk = id % a.chunks;
-  id /= a.chunks;
-  const int tile0 = a.tiles - 1 - id % a.tiles;  // the rows that see most come first
-  const int r = id / a.tiles;
-  const Request rq = request_of(a, r);
-  const int rows = rq.queries * share;
-  const int64_t bytes = (int64_t)a.block_size * D;  // of a block's head
+// The rows of a wavefront and what they have gathered: RT tiles of 16, row `first` + 16 t + c
+// in lanes with lane % 16 == c.
+template <typename T, bool FP8, int D, int RT, bool SPLIT>
+struct AttendRows {
+  static constexpr int CH = D / 64;  // 16-byte pieces of a key per lane
+  static constexpr int DT = D / 16;  // tiles of the output's dimensions
 
-  for (int tile = tile0; tile * ROWS < rows; tile += a.tiles) {
-    const int row0 = tile * ROWS, tile_end = last_key(rq, min(row0 + ROWS, rows) - 1, share);
-    const int pieces = min(max((tile_end + a.chunk_keys - 1) / a.chunk_keys, 1), a.chunks);
-    if (chunk >= pieces) continue;
-    const int first = row0 + (KS ? 0 : wave * RT * 16);  // this wavefront's rows
-    const int key0 = chunk * a.chunk_keys;
-    int key1 = first < rows ? last_key(rq, min(first + RT * 16, rows) - 1, share) : 0;
-    const int seen_by_any = key1, seen_by_all = first < rows ? last_key(rq, first, share) : 0;
-    if (chunk < pieces - 1) key1 = min(key1, key0 + a.chunk_keys);
-    if (a.num_blocks == 0) key1 = 0;
+  Operand q[RT][CH][2];  // dimensions ch * 64 + j * 16 + half * 8 + 0 ... 7
+  f32x4 o[RT][DT];       // dimension d * 16 + j * 4 + i
+  float top[RT], sum[RT];
+  int ends[RT], seen_by_all, seen_by_any;  // keys seen: by each row, by the first and the last
 
-    // queries: column c of the products, dimensions ch * 64 + j * 16 + half * 8 + 0 ... 7
-    Operand q[RT][CH][2];
-    int ends[RT];
+  __device__ __forceinline__ void begin(const AttendArgs& a, const Request& rq, int first, int rows, int kv, int share) {
+    const int c = lane_id() & 15, j = lane_id() >> 4;
+    seen_by_any = first < rows ? last_key(rq, min(first + RT * 16, rows) - 1, share) : 0;
+    seen_by_all = first < rows ? last_key(rq, first, share) : 0;
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
       const int row = first + t * 16 + c;
@@ -188,286 +172,415 @@ __global__ __launch_bounds__(kAttendWaves* kWave) void kv_attend_kernel(AttendAr
           q[t][ch][h] = Operand{};
           if (row < rows) q[t][ch][h] = *(const Operand*)(p + ch * 64 + j * 16 + h * 8);
         }
-    }
-
-    f32x4 o[RT][DT];
-    float top[RT], sum[RT];
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
       top[t] = -INFINITY, sum[t] = 0.0f;
 #pragma unroll
       for (int d = 0; d < DT; ++d) o[t][d] = f32x4{0, 0, 0, 0};
     }
+  }
 
-    const int stride = KS ? kAttendWaves * kStep : kStep;
-    const int begin = key0 + (KS ? wave * kStep : 0);
-    // which block holds 16 keys, and where in it they start
-    auto look_up = [&](int key, int* at) {
-      const uint32_t u = (uint32_t)key >> 4;
-      const uint32_t index = a.magic ? __umulhi(u, a.magic) : u;
-      *at = (int)(u - index * a.sixteenths) * 16;
-      return a.table[(int64_t)r * a.table_stride + min((int)index, a.width - 1)];
+  // 64 keys from kb on.  key(t, ch): 16 bytes of this lane's row of key tile t; value(d): the
+  // codes of its 16 keys in dimension d * 16 + c.  ks, vs: the scales of those keys' block (ks
+  // with the softmax's); valid: whether there is one.  keys_done() comes when the last key is used.
+  template <typename Key, typename Value, typename Done>
+  __device__ __forceinline__ void step(int kb, float ks, float vs, bool valid, Key key, Value value, Done keys_done) {
+    const int at16 = kb + (lane_id() >> 4) * 16;  // first of this lane's 16 keys
+    // a step that every row sees whole, of blocks that are all there, needs no masks
+    const bool whole = kb + kStep <= seen_by_all && __all(valid && ks >= 0.0f);
+    // values at keys that no row sees: whatever is there, its weight is 0 and must stay so
+    const int seen = valid ? min(max(seen_by_any - at16, 0), 16) : 0;
+    auto clean = [&](Vec<uint32_t, 4> v, bool nans) {
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const int n = min(max(seen - w * 4, 0), 4);
+        v.v[w] &= n == 4 ? 0xFFFFFFFFu : (1u << (8 * n)) - 1u;
+        if (FP8 && nans) v.v[w] &= ~nan_bytes(v.v[w]);
+      }
+      return v;
     };
+    if constexpr (FP8) {
+      if (!whole) {
+        // a NaN value at a key that some rows see and others do not: 0 * NaN would reach them
+        // all.  It is left out of the sums and counted by a product of its own.
+        uint32_t any = 0;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          const Vec<uint32_t, 4> v = clean(value(d), false);
+#pragma unroll
+          for (int w = 0; w < 4; ++w) any |= nan_bytes(v.v[w]);
+        }
+        if (__any(any != 0)) mark_nans(at16, valid, [&](int d) { return clean(value(d), false); });
+      }
+    }
+
+    f32x4 s[RT][4];
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt) {
+#pragma unroll
+      for (int t = 0; t < RT; ++t) s[t][kt] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int ch = 0; ch < CH; ++ch) {
+        const Vec<uint32_t, 4> w = key(kt, ch);
+        const Operand k0 = widen8<T, FP8>(w.v[0], w.v[1]), k1 = widen8<T, FP8>(w.v[2], w.v[3]);
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+          s[t][kt] = product<T>(k0, q[t][ch][0], s[t][kt]);
+          s[t][kt] = product<T>(k1, q[t][ch][1], s[t][kt]);
+        }
+      }
+    }
+    keys_done();
+
+    float unit = ks;  // what a score is still to be multiplied by
+    if (!whole) {
+      unit = 1.0f;
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[t][kt][i] = !valid || at16 + kt * 4 + i >= ends[t] ? -INFINITY : s[t][kt][i] * ks;
+    }
+    Operand hi[RT][2], lo[RT][2];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      float m = s[t][0][0];
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m = fmaxf(m, s[t][kt][i]);
+      m = groups_max(m * unit);
+      // weights may exceed 1 by 2^8 before the sums are brought to a new maximum: fp32 and
+      // bf16 keep their relative precision there
+      if (__any(m > top[t] + 8.0f)) {
+        const float now = fmaxf(top[t], m);
+        const float shrink = top[t] == -INFINITY ? 0.0f : exp2_fast(top[t] - now);
+        top[t] = now;
+        sum[t] *= shrink;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[t][d] *= shrink;
+      }
+      const float base = top[t] == -INFINITY ? 0.0f : top[t];
+      // the scale of a block that a row sees nothing of does not touch it, whatever it is
+      const float by = whole || (valid && at16 < ends[t]) ? vs : 0.0f;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float p0 = exp2_fast(fmaf(s[t][u * 2 + e / 2][(e % 2) * 2], unit, -base));
+          const float p1 = exp2_fast(fmaf(s[t][u * 2 + e / 2][(e % 2) * 2 + 1], unit, -base));
+          sum[t] += p0 + p1;
+          const float w0 = p0 * by, w1 = p1 * by;
+          hi[t][u].w[e] = pack_bf16x2(w0, w1);
+          if constexpr (SPLIT)
+            lo[t][u].w[e] = pack_bf16x2(w0 - u2f(hi[t][u].w[e] << 16), w1 - u2f(hi[t][u].w[e] & 0xFFFF0000u));
+        }
+    }
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+      Vec<uint32_t, 4> w = value(d);
+      if (!whole) w = clean(w, true);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const Operand v = widen8<BF16, FP8>(w.v[2 * u], w.v[2 * u + 1]);
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+          o[t][d] = product<BF16>(v, hi[t][u], o[t][d]);
+          if constexpr (SPLIT) o[t][d] = product<BF16>(v, lo[t][u], o[t][d]);
+        }
+      }
+    }
+  }
+
+  template <typename Value>
+  __device__ __forceinline__ void mark_nans(int at16, bool valid, Value value) {
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+      const Vec<uint32_t, 4> w = value(d);
+      uint32_t mark[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mark[i] = nan_bytes(w.v[i]) & 0x38383838u;  // 1.0 as e4m3
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+        f32x4 hit = {0, 0, 0, 0};
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          Operand p;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int key = at16 + u * 8 + e * 2;
+            p.w[e] = (valid && key < ends[t] ? 0x3F80u : 0u) | (valid && key + 1 < ends[t] ? 0x3F800000u : 0u);
+          }
+          hit = product<BF16>(widen8<BF16, true>(mark[2 * u], mark[2 * u + 1]), p, hit);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (hit[i] > 0.0f) o[t][d][i] = NAN;
+      }
+    }
+  }
+
+  __device__ __forceinline__ void finish() {
+#pragma unroll
+    for (int t = 0; t < RT; ++t) sum[t] = groups_sum(sum[t]);
+  }
+};
+
+// what a workgroup works on, from its number
+struct AttendUnit {
+  int kv, chunk, tile, r;
+  __device__ __forceinline__ AttendUnit(const AttendArgs& a) {
+    int id = blockIdx.x;
+    kv = id % a.kv_heads;
+    id /= a.kv_heads;
+    chunk = id % a.chunks;
+    id /= a.chunks;
+    tile = a.tiles - 1 - id % a.tiles;  // the rows that see most come first
+    r = id / a.tiles;
+  }
+};
+
+// the block of 16 keys from `key` on, and where in it they start
+__device__ __forceinline__ int look_up(const AttendArgs& a, int r, int key, int* at) {
+  const uint32_t u = (uint32_t)key >> 4;
+  const uint32_t index = a.magic ? __umulhi(u, a.magic) : u;
+  *at = (int)(u - index * a.sixteenths) * 16;
+  return a.table[(int64_t)r * a.table_stride + min((int)index, a.width - 1)];
+}
+__device__ __forceinline__ bool in_pool(const AttendArgs& a, int block) { return (uint32_t)block < (uint32_t)a.num_blocks; }
+__device__ __forceinline__ int64_t cell_of(const AttendArgs& a, int block, int kv) {
+  return (int64_t)(in_pool(a, block) ? block : 0) * a.kv_heads + kv;
+}
+
+// few rows: the wavefronts of a workgroup share them and split the keys; keys and values go
+// from memory into the registers they are multiplied from
+template <typename T, bool FP8, int D, int RT>
+__global__ __launch_bounds__(kAttendWaves* kWave, D == 256 || RT == 2 ? 1 : 2) void kv_attend_split_kernel(AttendArgs a) {
+  using Rows = AttendRows<T, FP8, D, RT, true>;
+  constexpr int ROWS = RT * 16, CH = Rows::CH, DT = Rows::DT;
+  const int lane = lane_id(), wave = threadIdx.x / kWave, c = lane & 15, j = lane >> 4;
+  const int share = a.q_heads / a.kv_heads;
+  const AttendUnit unit(a);
+  const int kv = unit.kv, chunk = unit.chunk, r = unit.r;
+  const Request rq = request_of(a, r);
+  const int rows = rq.queries * share;
+  const int64_t bytes = (int64_t)a.block_size * D;  // of a block's head
+  __shared__ float meet_top[kAttendWaves][ROWS], meet_sum[kAttendWaves][ROWS];
+  __shared__ float meet_o[kAttendWaves][16][D + 4];
+
+  for (int tile = unit.tile; tile * ROWS < rows; tile += a.tiles) {
+    const int first = tile * ROWS, tile_end = last_key(rq, min(first + ROWS, rows) - 1, share);
+    const int pieces = min(max((tile_end + a.chunk_keys - 1) / a.chunk_keys, 1), a.chunks);
+    if (chunk >= pieces) continue;
+    Rows w;
+    w.begin(a, rq, first, rows, kv, share);
+    const int key0 = chunk * a.chunk_keys + wave * kStep;
+    int key1 = a.num_blocks ? tile_end : 0;
+    if (chunk < pieces - 1) key1 = min(key1, (chunk + 1) * a.chunk_keys);
+
+    constexpr int STRIDE = kAttendWaves * kStep;
     Vec<uint32_t, 4> kw[4][CH], vw[DT];
     float ks = 0.0f, vs = 0.0f;
-    int bk, ak, bv, av;  // block and position: of the keys this lane multiplies, of those it gets
+    int bk = 0, ak = 0, bv = 0, av = 0;  // block and position: of the keys this lane multiplies, of those it gets
     auto load_keys = [&](int block, int at) {
-      block = (uint32_t)block < (uint32_t)a.num_blocks ? block : 0;
-      const uint8_t* p = a.key + ((int64_t)block * a.kv_heads + kv) * bytes + (at + (c & 3)) * D + j * 16;
+      const uint8_t* p = a.key + cell_of(a, block, kv) * bytes + (at + (c & 3)) * D + j * 16;
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int ch = 0; ch < CH; ++ch) kw[t][ch] = ldg_nt<uint32_t, 4>((const uint32_t*)(p + t * 4 * D + ch * 64));
     };
     auto load_scales = [&](int block) {
-      block = (uint32_t)block < (uint32_t)a.num_blocks ? block : 0;
-      ks = a.key_scale[(int64_t)block * a.kv_heads + kv];
-      vs = a.value_scale[(int64_t)block * a.kv_heads + kv];
+      ks = a.key_scale[cell_of(a, block, kv)];
+      vs = a.value_scale[cell_of(a, block, kv)];
     };
     auto load_values = [&](int block, int at) {
-      block = (uint32_t)block < (uint32_t)a.num_blocks ? block : 0;
-      const uint8_t* p = a.value + ((int64_t)block * a.kv_heads + kv) * bytes + c * a.block_size + at;
+      const uint8_t* p = a.value + cell_of(a, block, kv) * bytes + c * a.block_size + at;
 #pragma unroll
       for (int d = 0; d < DT; ++d) vw[d] = ldg_nt<uint32_t, 4>((const uint32_t*)(p + d * 16 * a.block_size));
     };
-    if (begin < key1) {
-      bk = look_up(begin + (c >> 2) * 16, &ak);
-      bv = look_up(begin + j * 16, &av);
+    if (key0 < key1) {
+      bk = look_up(a, r, key0 + (c >> 2) * 16, &ak);
+      bv = look_up(a, r, key0 + j * 16, &av);
       load_keys(bk, ak);
       load_scales(bv);
       load_values(bv, av);
     }
-    for (int kb = begin; kb < key1; kb += stride) {
-      const bool more = kb + stride < key1;
-      const bool valid = (uint32_t)bv < (uint32_t)a.num_blocks;
+    for (int kb = key0; kb < key1; kb += STRIDE) {
+      const bool more = kb + STRIDE < key1;
+      const bool valid = in_pool(a, bv);
       const float ks_now = ks * a.scale, vs_now = vs;
-      const int at16 = kb + j * 16;  // first of this lane's 16 keys
-      int bk1 = 0, ak1 = 0, bv1 = 0, av1 = 0;
       if (more) {
-        bk1 = look_up(kb + stride + (c >> 2) * 16, &ak1);
-        bv1 = look_up(kb + stride + j * 16, &av1);
+        bk = look_up(a, r, kb + STRIDE + (c >> 2) * 16, &ak);
+        bv = look_up(a, r, kb + STRIDE + j * 16, &av);
       }
-      f32x4 s[RT][4];
-#pragma unroll
-      for (int kt = 0; kt < 4; ++kt) {
-#pragma unroll
-        for (int t = 0; t < RT; ++t) s[t][kt] = f32x4{0, 0, 0, 0};
-#pragma unroll
-        for (int ch = 0; ch < CH; ++ch) {
-          const Operand k0 = widen8<T, FP8>(kw[kt][ch].v[0], kw[kt][ch].v[1]);
-          const Operand k1 = widen8<T, FP8>(kw[kt][ch].v[2], kw[kt][ch].v[3]);
-#pragma unroll
-          for (int t = 0; t < RT; ++t) {
-            s[t][kt] = product<T>(k0, q[t][ch][0], s[t][kt]);
-            s[t][kt] = product<T>(k1, q[t][ch][1], s[t][kt]);
-          }
-        }
-      }
-      if (more) {
-        load_keys(bk1, ak1);
-        load_scales(bv1);
-      }
-      // a step that every row sees whole skips all of this
-      const bool whole = kb + kStep <= seen_by_all && __all(valid);
-      if (!whole) {
-#pragma unroll
-        for (int t = 0; t < RT; ++t)
-#pragma unroll
-          for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (!valid || at16 + kt * 4 + i >= ends[t]) s[t][kt][i] = -INFINITY;
-              else s[t][kt][i] *= ks_now;
-        // values at keys that no row sees: whatever is there, its weight is 0 and must stay so
-        const int seen = valid ? min(max(seen_by_any - at16, 0), 16) : 0;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const int n = min(max(seen - w * 4, 0), 4);
-          const uint32_t keep = n == 4 ? 0xFFFFFFFFu : (1u << (8 * n)) - 1u;
-#pragma unroll
-          for (int d = 0; d < DT; ++d) vw[d].v[w] &= keep;
-        }
-        if constexpr (FP8) {
-          // a NaN value at a key that some rows see and others do not: 0 * NaN would reach
-          // them all.  Take it out and count it by a product of its own.
-          uint32_t any = 0;
-#pragma unroll
-          for (int d = 0; d < DT; ++d)
-#pragma unroll
-            for (int w = 0; w < 4; ++w) any |= nan_bytes(vw[d].v[w]);
-          if (__any(any != 0)) {
-#pragma unroll
-            for (int d = 0; d < DT; ++d) {
-              uint32_t mark[4];
-#pragma unroll
-              for (int w = 0; w < 4; ++w) {
-                const uint32_t n = nan_bytes(vw[d].v[w]);
-                vw[d].v[w] &= ~n;
-                mark[w] = n & 0x38383838u;  // 1.0 as e4m3
-              }
-#pragma unroll
-              for (int t = 0; t < RT; ++t) {
-                f32x4 hit = {0, 0, 0, 0};
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                  Operand p;
-#pragma unroll
-                  for (int e = 0; e < 4; ++e) {
-                    const int key = at16 + u * 8 + e * 2;
-                    p.w[e] = (valid && key < ends[t] ? 0x3F80u : 0u) | (valid && key + 1 < ends[t] ? 0x3F800000u : 0u);
-                  }
-                  hit = product<BF16>(widen8<BF16, true>(mark[2 * u], mark[2 * u + 1]), p, hit);
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                  if (hit[i] > 0.0f) o[t][d][i] = NAN;
-              }
-            }
-          }
-        }
-      } else {
-#pragma unroll
-        for (int t = 0; t < RT; ++t)
-#pragma unroll
-          for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s[t][kt][i] *= ks_now;
-      }
-
-      Operand hi[RT][2], lo[RT][2];
-#pragma unroll
-      for (int t = 0; t < RT; ++t) {
-        float m = s[t][0][0];
-#pragma unroll
-        for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) m = fmaxf(m, s[t][kt][i]);
-        m = groups_max(m);
-        // weights may exceed 1 by 2^8 before the sums are brought to a new maximum: fp32 and
-        // bf16 keep their relative precision there
-        if (__any(m > top[t] + 8.0f)) {
-          const float now = fmaxf(top[t], m);
-          const float shrink = top[t] == -INFINITY ? 0.0f : exp2_fast(top[t] - now);
-          top[t] = now;
-          sum[t] *= shrink;
-#pragma unroll
-          for (int d = 0; d < DT; ++d) o[t][d] *= shrink;
-        }
-        const float base = top[t] == -INFINITY ? 0.0f : top[t];
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float p0 = exp2_fast(s[t][u * 2 + e / 2][(e % 2) * 2] - base);
-            const float p1 = exp2_fast(s[t][u * 2 + e / 2][(e % 2) * 2 + 1] - base);
-            sum[t] += p0 + p1;
-            // a hidden key's weight is 0 whatever its block's scale
-            const float w0 = p0 == 0.0f ? 0.0f : p0 * vs_now, w1 = p1 == 0.0f ? 0.0f : p1 * vs_now;
-            hi[t][u].w[e] = pack_bf16x2(w0, w1);
-            if constexpr (SPLIT)
-              lo[t][u].w[e] = pack_bf16x2(w0 - u2f(hi[t][u].w[e] << 16), w1 - u2f(hi[t][u].w[e] & 0xFFFF0000u));
-          }
-      }
-#pragma unroll
-      for (int d = 0; d < DT; ++d) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const Operand v = widen8<BF16, FP8>(vw[d].v[2 * u], vw[d].v[2 * u + 1]);
-#pragma unroll
-          for (int t = 0; t < RT; ++t) {
-            o[t][d] = product<BF16>(v, hi[t][u], o[t][d]);
-            if constexpr (SPLIT) o[t][d] = product<BF16>(v, lo[t][u], o[t][d]);
-          }
-        }
-      }
-      if (more) load_values(bv1, av1);
-      bv = bv1;
+      w.step(kb, ks_now, vs_now, valid, [&](int t, int ch) { return kw[t][ch]; }, [&](int d) { return vw[d]; },
+             [&] {
+               if (more) {
+                 load_keys(bk, ak);
+                 load_scales(bv);
+               }
+             });
+      if (more) load_values(bv, av);
     }
-#pragma unroll
-    for (int t = 0; t < RT; ++t) sum[t] = groups_sum(sum[t]);
+    w.finish();
 
-    if constexpr (KS) {
-      // the wavefronts bring their sums to the common maximum and add them in LDS
-      __shared__ float meet_top[kAttendWaves][RT * 16], meet_sum[kAttendWaves][RT * 16];
-      __shared__ float meet_o[kAttendWaves][16][D + 4];
-      if (j == 0) {
+    // the wavefronts bring their sums to the common maximum and add them in LDS
+    if (j == 0) {
 #pragma unroll
-        for (int t = 0; t < RT; ++t) meet_top[wave][t * 16 + c] = top[t], meet_sum[wave][t * 16 + c] = sum[t];
-      }
+      for (int t = 0; t < RT; ++t) meet_top[wave][t * 16 + c] = w.top[t], meet_sum[wave][t * 16 + c] = w.sum[t];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      float all = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < kAttendWaves; ++i) all = fmaxf(all, meet_top[i][t * 16 + c]);
+      const float mine = w.top[t] == -INFINITY ? 0.0f : exp2_fast(w.top[t] - all);
+#pragma unroll
+      for (int d = 0; d < DT; ++d) *(f32x4*)&meet_o[wave][c][d * 16 + j * 4] = w.o[t][d] * mine;
       __syncthreads();
+      // 16 threads a row, 4 numbers at a time
+      const int row_in = threadIdx.x / 16, piece = threadIdx.x % 16, row = first + t * 16 + row_in;
+      float row_top = -INFINITY, row_sum = 0.0f;
 #pragma unroll
-      for (int t = 0; t < RT; ++t) {
-        float all = -INFINITY, total = 0.0f;
+      for (int i = 0; i < kAttendWaves; ++i) row_top = fmaxf(row_top, meet_top[i][t * 16 + row_in]);
 #pragma unroll
-        for (int w = 0; w < kAttendWaves; ++w) all = fmaxf(all, meet_top[w][t * 16 + c]);
-#pragma unroll
-        for (int w = 0; w < kAttendWaves; ++w) {
-          const float m = meet_top[w][t * 16 + c];
-          if (m != -INFINITY) total += meet_sum[w][t * 16 + c] * exp2_fast(m - all);
-        }
-        const float mine = top[t] == -INFINITY ? 0.0f : exp2_fast(top[t] - all);
-#pragma unroll
-        for (int d = 0; d < DT; ++d) {
-          const f32x4 v = o[t][d] * mine;
-          *(f32x4*)&meet_o[wave][c][d * 16 + j * 4] = v;
-        }
-        __syncthreads();
-        // 16 rows x D: 16 threads a row, 4 numbers at a time; the row's maximum and sum come
-        // from a lane that has them (lane % 16 is the row there)
-        const int row_in = threadIdx.x / 16, piece = threadIdx.x % 16;
-        float row_all = -INFINITY, row_total = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kAttendWaves; ++w) row_all = fmaxf(row_all, meet_top[w][t * 16 + row_in]);
-#pragma unroll
-        for (int w = 0; w < kAttendWaves; ++w) {
-          const float m = meet_top[w][t * 16 + row_in];
-          if (m != -INFINITY) row_total += meet_sum[w][t * 16 + row_in] * exp2_fast(m - row_all);
-        }
-        const int row = first + t * 16 + row_in;
-        if (row < rows) {
-          const int64_t cell = (int64_t)(rq.q0 + row / share) * a.q_heads + kv * share + row % share;
-#pragma unroll
-          for (int x = 0; x < D / 64; ++x) {
-            f32x4 v = {0, 0, 0, 0};
-#pragma unroll
-            for (int w = 0; w < kAttendWaves; ++w) v += *(const f32x4*)&meet_o[w][row_in][x * 64 + piece * 4];
-            if (pieces == 1) {
-              const float by = row_total == 0.0f ? 0.0f : 1.0f / row_total;
-              Vec<uint16_t, 4> h;
-#pragma unroll
-              for (int e = 0; e < 4; ++e) h.v[e] = T::from_f32(row_total == 0.0f ? 0.0f : v[e] * by);
-              stg(a.out + cell * D + x * 64 + piece * 4, h);
-            } else {
-              const int64_t at = (int64_t)chunk * a.tokens * a.q_heads + cell;
-              *(f32x4*)(a.part_o + at * D + x * 64 + piece * 4) = v;
-              if (x == 0 && piece == 0) a.part_ml[at * 2] = row_all, a.part_ml[at * 2 + 1] = row_total;
-            }
-          }
-        }
-        __syncthreads();
-        (void)total;
+      for (int i = 0; i < kAttendWaves; ++i) {
+        const float m = meet_top[i][t * 16 + row_in];
+        row_sum += meet_sum[i][t * 16 + row_in] * (m == -INFINITY ? 1.0f : exp2_fast(m - row_top));
       }
-    } else {
-#pragma unroll
-      for (int t = 0; t < RT; ++t) {
-        const int row = first + t * 16 + c;
-        if (row >= rows) continue;
+      if (row < rows) {
         const int64_t cell = (int64_t)(rq.q0 + row / share) * a.q_heads + kv * share + row % share;
-        if (pieces == 1) {
-          const float by = sum[t] == 0.0f ? 0.0f : 1.0f / sum[t];
 #pragma unroll
-          for (int d = 0; d < DT; ++d) {
+        for (int x = 0; x < D / 64; ++x) {
+          f32x4 v = {0, 0, 0, 0};
+#pragma unroll
+          for (int i = 0; i < kAttendWaves; ++i) v += *(const f32x4*)&meet_o[i][row_in][x * 64 + piece * 4];
+          if (pieces == 1) {
+            const float by = row_sum == 0.0f ? 0.0f : 1.0f / row_sum;
             Vec<uint16_t, 4> h;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) h.v[e] = T::from_f32(sum[t] == 0.0f ? 0.0f : o[t][d][e] * by);
-            stg(a.out + cell * D + d * 16 + j * 4, h);
+            for (int e = 0; e < 4; ++e) h.v[e] = T::from_f32(row_sum == 0.0f ? 0.0f : v[e] * by);
+            stg(a.out + cell * D + x * 64 + piece * 4, h);
+          } else {
+            const int64_t at = (int64_t)chunk * a.tokens * a.q_heads + cell;
+            *(f32x4*)(a.part_o + at * D + x * 64 + piece * 4) = v;
+            if (x == 0 && piece == 0) a.part_ml[at * 2] = row_top, a.part_ml[at * 2 + 1] = row_sum;
           }
-        } else {
-          const int64_t at = (int64_t)chunk * a.tokens * a.q_heads + cell;
-#pragma unroll
-          for (int d = 0; d < DT; ++d) *(f32x4*)(a.part_o + at * D + d * 16 + j * 4) = o[t][d];
-          if (j == 0) a.part_ml[at * 2] = top[t], a.part_ml[at * 2 + 1] = sum[t];
         }
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// many rows: each wavefront has its own, and the workgroup reads the keys and values once,
+// 64 keys ahead, into LDS.  A lane's operand is 16 bytes of a row of its own: read from memory
+// directly that is one cache line a lane, and the lines a cycle are what bound the kernel
+// (measured at 2 x 2000 queries over 4000 keys: 455 us).  Pieces of a row are swapped in LDS
+// by some bits of the row's number, so that the rows that are read together lie in different
+// banks.
+template <typename T, bool FP8, int D, int RT, bool SPLIT>
+__global__ __launch_bounds__(kAttendWaves* kWave, D == 256 ? 1 : 2) void kv_attend_rows_kernel(AttendArgs a) {
+  using Rows = AttendRows<T, FP8, D, RT, SPLIT>;
+  constexpr int ROWS = kAttendWaves * RT * 16, PIECES = D / 64;  // 16-byte pieces a thread loads of either
+  constexpr int KP = D / 16;                                     // pieces of a key
+  constexpr int KEYS = kAttendWaves * kWave / KP;                // keys per round of loads
+  const int lane = lane_id(), wave = threadIdx.x / kWave, c = lane & 15, j = lane >> 4;
+  const int share = a.q_heads / a.kv_heads;
+  const AttendUnit unit(a);
+  const int kv = unit.kv, chunk = unit.chunk, r = unit.r;
+  const Request rq = request_of(a, r);
+  const int rows = rq.queries * share;
+  const int64_t bytes = (int64_t)a.block_size * D;
+  __shared__ Vec<uint32_t, 4> keys[2][kStep * KP], values[2][D * 4];
+  auto key_place = [](int key, int piece) { return key * KP + (piece ^ (((key & 3) | ((key >> 4) & 1) << 2) & (KP - 1))); };
+  auto value_place = [](int d, int group) { return d * 4 + (group ^ ((d >> 2) & 3)); };
+
+  for (int tile = unit.tile; tile * ROWS < rows; tile += a.tiles) {
+    const int row0 = tile * ROWS, tile_end = last_key(rq, min(row0 + ROWS, rows) - 1, share);
+    const int pieces = min(max((tile_end + a.chunk_keys - 1) / a.chunk_keys, 1), a.chunks);
+    if (chunk >= pieces) continue;
+    const int first = row0 + wave * RT * 16;
+    Rows w;
+    w.begin(a, rq, first, rows, kv, share);
+    const int key0 = chunk * a.chunk_keys;
+    int key1 = a.num_blocks ? tile_end : 0;
+    if (chunk < pieces - 1) key1 = min(key1, key0 + a.chunk_keys);
+
+    Vec<uint32_t, 4> kr[PIECES], vr[PIECES];
+    float ks = 0.0f, vs = 0.0f;
+    int bk[PIECES], ak[PIECES], bv, av, bs_next = 0;  // blocks of the step to load; bs: of this lane's 16 keys
+    const int my_key = threadIdx.x / KP, my_piece = threadIdx.x % KP, my_group = threadIdx.x % 4, my_d = threadIdx.x / 4;
+    auto find = [&](int kb) {
+#pragma unroll
+      for (int p = 0; p < PIECES; ++p) {
+        const int key = kb + my_key + p * KEYS;
+        bk[p] = look_up(a, r, key, &ak[p]);
+        ak[p] += key & 15;
+      }
+      bv = look_up(a, r, kb + my_group * 16, &av);
+    };
+    auto load = [&] {
+#pragma unroll
+      for (int p = 0; p < PIECES; ++p)
+        kr[p] = ldg<uint32_t, 4>((const uint32_t*)(a.key + cell_of(a, bk[p], kv) * bytes + ak[p] * D + my_piece * 16));
+      const uint8_t* v = a.value + cell_of(a, bv, kv) * bytes + my_d * a.block_size + av;
+#pragma unroll
+      for (int p = 0; p < PIECES; ++p) vr[p] = ldg<uint32_t, 4>((const uint32_t*)(v + p * 64 * a.block_size));
+      bs_next = __shfl(bv, j, kWave);  // lane j's group is j
+      ks = a.key_scale[cell_of(a, bs_next, kv)] * a.scale;
+      vs = a.value_scale[cell_of(a, bs_next, kv)];
+    };
+    auto store = [&](int half) {
+#pragma unroll
+      for (int p = 0; p < PIECES; ++p) {
+        keys[half][key_place(my_key + p * KEYS, my_piece)] = kr[p];
+        values[half][value_place(my_d + p * 64, my_group)] = vr[p];
+      }
+    };
+    __syncthreads();  // the tile before may still be read
+    if (key0 < key1) {
+      find(key0);
+      load();
+      find(key0 + kStep);
+      store(0);
+    }
+    __syncthreads();
+    int half = 0;
+    for (int kb = key0; kb < key1; kb += kStep, half ^= 1) {
+      const float ks_now = ks, vs_now = vs;
+      const bool valid = in_pool(a, bs_next), more = kb + kStep < key1;
+      if (more) {
+        load();
+        find(kb + 2 * kStep);
+      }
+      if (kb < w.seen_by_any)
+        w.step(kb, ks_now, vs_now, valid,
+               [&](int t, int ch) { return keys[half][key_place((c >> 2) * 16 + t * 4 + (c & 3), ch * 4 + j)]; },
+               [&](int d) { return values[half][value_place(d * 16 + c, j)]; }, [] {});
+      if (more) store(half ^ 1);
+      __syncthreads();
+    }
+    w.finish();
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      const int row = first + t * 16 + c;
+      if (row >= rows) continue;
+      const int64_t cell = (int64_t)(rq.q0 + row / share) * a.q_heads + kv * share + row % share;
+      if (pieces == 1) {
+        const float by = w.sum[t] == 0.0f ? 0.0f : 1.0f / w.sum[t];
+#pragma unroll
+        for (int d = 0; d < Rows::DT; ++d) {
+          Vec<uint16_t, 4> h;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) h.v[e] = T::from_f32(w.sum[t] == 0.0f ? 0.0f : w.o[t][d][e] * by);
+          stg(a.out + cell * D + d * 16 + j * 4, h);
+        }
+      } else {
+        const int64_t at = (int64_t)chunk * a.tokens * a.q_heads + cell;
+#pragma unroll
+        for (int d = 0; d < Rows::DT; ++d) *(f32x4*)(a.part_o + at * D + d * 16 + j * 4) = w.o[t][d];
+        if (j == 0) a.part_ml[at * 2] = w.top[t], a.part_ml[at * 2 + 1] = w.sum[t];
       }
     }
   }
@@ -491,19 +604,36 @@ __global__ __launch_bounds__(kAttendWaves* kWave) void kv_attend_join_kernel(Att
     const int pieces = min(max((tile_end + a.chunk_keys - 1) / a.chunk_keys, 1), a.chunks);
     if (pieces == 1) continue;
     const int64_t cell = (int64_t)(rq.q0 + i) * a.q_heads + head, step = (int64_t)a.tokens * a.q_heads;
-    float top = -INFINITY, sum = 0.0f, o[PER] = {};
-    for (int p = 0; p < pieces; ++p) top = fmaxf(top, a.part_ml[(p * step + cell) * 2]);
-    for (int p = 0; p < pieces; ++p) {
-      const int64_t at = p * step + cell;
-      const float m = a.part_ml[at * 2];
-      if (m == -INFINITY) {
-        sum += a.part_ml[at * 2 + 1];  // 0, or NaN where every score was
-        continue;
-      }
-      const float w = exp2_fast(m - top);
-      sum += w * a.part_ml[at * 2 + 1];
+    // lane p holds the weight of chunk p; 64 at a time
+    float top = -INFINITY;
+    for (int p = lane; p < pieces; p += kWave) top = fmaxf(top, a.part_ml[(p * step + cell) * 2]);
 #pragma unroll
-      for (int e = 0; e < PER; ++e) o[e] += w * a.part_o[at * D + lane * PER + e];
+    for (int m = 1; m < kWave; m *= 2) top = fmaxf(top, wave_shfl_xor(top, m));
+    float sum = 0.0f, o[PER] = {};
+    for (int p0 = 0; p0 < pieces; p0 += kWave) {
+      float w = 0.0f, part = 0.0f;
+      if (p0 + lane < pieces) {
+        const int64_t at = ((p0 + lane) * step + cell) * 2;
+        const float m = a.part_ml[at];
+        w = m == -INFINITY ? 0.0f : exp2_fast(m - top);
+        part = a.part_ml[at + 1] * (m == -INFINITY ? 1.0f : w);  // a chunk without a maximum: 0, or NaN
+      }
+#pragma unroll
+      for (int m = 1; m < kWave; m *= 2) part += wave_shfl_xor(part, m);
+      sum += part;
+      const int n = min(pieces - p0, kWave);
+      for (int p = 0; p < n; p += 8) {
+        Vec<float, PER> v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)  // the last ones again, with no weight, behind the last
+          v[e] = ldg<float, PER>(a.part_o + ((p0 + min(p + e, n - 1)) * step + cell) * D + lane * PER);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float by = p + e < n ? __shfl(w, p + e, kWave) : 0.0f;
+#pragma unroll
+          for (int x = 0; x < PER; ++x) o[x] = by == 0.0f ? o[x] : fmaf(by, v[e].v[x], o[x]);
+        }
+      }
     }
     const float by = sum == 0.0f ? 0.0f : 1.0f / sum;
     Vec<uint16_t, PER> h;
@@ -528,14 +658,20 @@ Launch plan_launch(int64_t requests, int32_t q_heads, int32_t kv_heads, int32_t 
   l.row_tiles = head_dim == 256 || rows <= 16 ? 1 : 2;
   l.tile_rows = (l.split_keys ? 1 : kAttendWaves) * l.row_tiles * 16;
   l.tiles = cdiv(rows, l.tile_rows);
-  const int64_t units = requests * kv_heads * l.tiles, wanted = 1024;
-  const int64_t floor_keys = l.split_keys ? 512 : 1024, cap = 8192;
-  int64_t keys = cdiv(cdiv(max_seq * units, wanted), 256) * 256;
-  if (keys < floor_keys) keys = floor_keys;
-  if (keys > cap) keys = cap;
-  l.chunk_keys = keys;
-  l.chunks = cdiv(max_seq, keys);
-  if (!l.split_keys && units >= wanted / 2) l.chunks = 1, l.chunk_keys = 1 << 30;
+  // As many workgroups as are resident at once (two per compute unit), in one go: with 512 of
+  // them 64 x 4096 takes 81 to 88 us, with 768 121 and with 1024 to 2048 89 to 98.  Chunks
+  // below kFloor keys cost more to bring together than they gain.
+  constexpr int64_t kResident = 512, kFloor = 256;
+  const int64_t units = requests * kv_heads * l.tiles;
+  int64_t chunks = kResident / (units < kResident ? units : kResident);
+  // a chunk's sums leave and come back in fp32: not for more rows than the keys they stand for
+  if (!l.split_keys && units >= kResident / 2) chunks = 1;
+  int64_t keys = cdiv(cdiv(max_seq, chunks), 256) * 256;
+  if (keys < kFloor) keys = kFloor;
+  l.chunk_keys = chunks == 1 && !l.split_keys ? 1 << 30 : keys;
+  // requests of very different lengths: the long ones are cut further
+  if (l.split_keys && l.chunk_keys > 8192) l.chunk_keys = 8192;
+  l.chunks = cdiv(max_seq, l.chunk_keys);
   return l;
 }
 
@@ -603,15 +739,12 @@ extern "C" int ctmi_kv_attend(const void* q, int32_t dtype, int64_t q_token_stri
   const bool fp8 = blocks->code_dtype == CTMI_F8E4M3;
   // bf16 outputs of long prompts take the weights as one bf16 number (2^-8, half a step of the
   // output's type); elsewhere they are two, which costs nothing while memory is the bound
-#define LAUNCH(T, F, D, RT, KS) kv_attend_kernel<T, F, D, RT, KS, KS || T::id == CTMI_F16><<<blocks_of, threads, 0, s>>>(a)
-#define BY_TILE(T, F, D)                                          \
-  do {                                                            \
-    if (l.split_keys) {                                           \
-      if (D == 256 || l.row_tiles == 1) LAUNCH(T, F, D, 1, true); \
-      else LAUNCH(T, F, D, (D == 256 ? 1 : 2), true);             \
-    } else {                                                      \
-      LAUNCH(T, F, D, (D == 256 ? 1 : 2), false);                 \
-    }                                                             \
+#define BY_TILE(T, F, D)                                                                                           \
+  do {                                                                                                             \
+    constexpr int RT2 = D == 256 ? 1 : 2;                                                                          \
+    if (!l.split_keys) kv_attend_rows_kernel<T, F, D, RT2, T::id == CTMI_F16><<<blocks_of, threads, 0, s>>>(a);    \
+    else if (RT2 == 1 || l.row_tiles == 1) kv_attend_split_kernel<T, F, D, 1><<<blocks_of, threads, 0, s>>>(a);    \
+    else kv_attend_split_kernel<T, F, D, RT2><<<blocks_of, threads, 0, s>>>(a);                                    \
     if (cells) kv_attend_join_kernel<T, D><<<dim3((unsigned)join), threads, 0, s>>>(a, l.tile_rows, (int)max_query); \
   } while (0)
 #define BY_CODE(T, D) do { if (fp8) BY_TILE(T, true, D); else BY_TILE(T, false, D); } while (0)
@@ -621,6 +754,5 @@ extern "C" int ctmi_kv_attend(const void* q, int32_t dtype, int64_t q_token_stri
 #undef BY_DIM
 #undef BY_CODE
 #undef BY_TILE
-#undef LAUNCH
   return check_launch("kv_attend");
 }
