@@ -494,24 +494,28 @@ def ptr(t: Optional[torch.Tensor]) -> Optional[int]:
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
-class _SameDevice:
-    """a context that changes nothing"""
+def gpu_index(first: torch.Tensor, *others: Optional[torch.Tensor]) -> int:
+    """require_gpu for the calls of a serving step, a fifth of its cost: the number of the GPU
+    all given tensors sit on"""
+    index = first.get_device()
+    if index < 0:
+        require_gpu(first)
+    for t in others:
+        if t is not None and t.get_device() != index:
+            require_gpu(first, *others)
+    return index
 
-    def __enter__(self):
-        return None
 
-    def __exit__(self, *exc):
-        return None
-
-
-_SAME_DEVICE = _SameDevice()
+def is_current(index: int) -> bool:
+    """whether kernels and allocations go to GPU `index` as things stand"""
+    return index == torch._C._cuda_getDevice()
 
 
-def on_device(device: torch.device):
-    """context in which kernels and allocations go to `device` (free where it is current)"""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return _SAME_DEVICE
-    return torch.cuda.device(device)
+def stream_of_index(index: int) -> int:
+    """stream_of for a device's number"""
+    if _raw_stream is not None:
+        return _raw_stream(index)
+    return torch.cuda.current_stream(index).cuda_stream
 
 
 def stream_of(device: torch.device) -> int:

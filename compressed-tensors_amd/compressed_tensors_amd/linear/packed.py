@@ -61,24 +61,25 @@ def packed_linear(x: Tensor, weight_packed: Tensor, weight_scale: Tensor,
         if bias.dtype is not x.dtype or tuple(bias.shape) != (n,):
             raise ValueError(f"expected a bias {x.dtype} [{n}], got {bias.dtype} {tuple(bias.shape)}")
         bias = bias.contiguous()
-    device = _lib.require_gpu(x, weight_packed, weight_scale, weight_zero_point, bias)
+    index = _lib.gpu_index(x, weight_packed, weight_scale, weight_zero_point, bias)
+    if not _lib.is_current(index):
+        with torch.cuda.device(index):
+            return packed_linear(x, weight_packed, weight_scale, weight_zero_point, bias)
     if weight_scale.dtype is not x.dtype and weight_scale.dtype is not torch.float32:
         weight_scale = weight_scale.float()
     weight_packed, weight_scale = weight_packed.contiguous(), weight_scale.contiguous()
     rows = x if x.ndim == 2 else x.reshape(-1, k)
+    m, (stride, inner) = rows.shape[0], rows.stride()
     # rows that start at 16-byte boundaries are read in place
-    if (rows.stride(1) != 1 or rows.stride(0) % 8 or rows.data_ptr() % 16
-            or (rows.shape[0] > 1 and not k <= rows.stride(0) < 1 << 24)):
-        rows = torch.empty((rows.shape[0], (k + 7) // 8 * 8), dtype=x.dtype, device=device)[:, :k].copy_(rows)
-    m = rows.shape[0]
+    if inner != 1 or stride % 8 or rows.data_ptr() % 16 or (m > 1 and not k <= stride < 1 << 24):
+        rows = x.new_empty((m, (k + 7) // 8 * 8))[:, :k].copy_(rows)
+        stride = rows.stride(0)
     lib = _lib.load()
-    with _lib.on_device(device):
-        out = torch.empty((*x.shape[:-1], n), dtype=x.dtype, device=device)
-        tmp_bytes = lib.ctmi_packed_linear_tmp_bytes(m, n, k, k // groups)
-        tmp = torch.empty(tmp_bytes, dtype=torch.uint8, device=device) if tmp_bytes else None
-        _lib.check(lib.ctmi_packed_linear(
-            rows.data_ptr(), _lib.dtype_code(x.dtype), rows.stride(0), weight_packed.data_ptr(),
-            weight_scale.data_ptr(), _lib.dtype_code(weight_scale.dtype), _lib.ptr(weight_zero_point),
-            _lib.ptr(bias), out.data_ptr(), m, n, k, k // groups, _lib.ptr(tmp), tmp_bytes,
-            _lib.stream_of(device)))
+    out = x.new_empty((m, n) if x.ndim == 2 else (*x.shape[:-1], n))
+    tmp_bytes = lib.ctmi_packed_linear_tmp_bytes(m, n, k, k // groups)
+    tmp = torch.empty(tmp_bytes, dtype=torch.uint8, device=x.device) if tmp_bytes else None
+    _lib.check(lib.ctmi_packed_linear(
+        rows.data_ptr(), _lib.dtype_code(x.dtype), stride, weight_packed.data_ptr(), weight_scale.data_ptr(),
+        _lib.dtype_code(weight_scale.dtype), _lib.ptr(weight_zero_point), _lib.ptr(bias), out.data_ptr(), m, n, k,
+        k // groups, _lib.ptr(tmp), tmp_bytes, _lib.stream_of_index(index)))
     return out

@@ -58,7 +58,7 @@ def _describe(blocks: KVBlocks) -> _lib.KVBlocksC:
     if key.ndim != 4:
         raise ValueError(f"expected keys [blocks, heads, block size, head dim], got {tuple(key.shape)}")
     n, heads, size, dim = key.shape
-    if tuple(value.shape) != (n, heads, dim, size):
+    if value.shape != (n, heads, dim, size):
         raise ValueError(f"expected values {(n, heads, dim, size)}, got {tuple(value.shape)}")
     if key_scale.shape != (n, heads) or value_scale.shape != (n, heads):
         raise ValueError(f"expected scales {(n, heads)}, got {tuple(key_scale.shape)} and {tuple(value_scale.shape)}")
@@ -76,12 +76,11 @@ def _describe(blocks: KVBlocks) -> _lib.KVBlocksC:
                           n, heads, dim, size, _lib.dtype_code(key.dtype))
 
 
-def _int_tensor(name: str, t: Tensor, dtype: torch.dtype, *shape) -> Tensor:
-    """`t`, contiguous, after a check of its type and shape (None in `shape`: any size)"""
-    if t.dtype is not dtype or t.ndim != len(shape) or any(s is not None and s != d for s, d in zip(shape, t.shape)):
-        want = ", ".join("*" if s is None else str(s) for s in shape)
-        raise ValueError(f"{name}: expected {dtype} [{want}], got {t.dtype} {tuple(t.shape)}")
-    return t if t.is_contiguous() else t.contiguous()
+def _ints(name: str, t: Tensor, dtype: torch.dtype, count: Optional[int] = None) -> Tensor:
+    """`t`, contiguous, after a check that it is a list of `count` (None: any number) integers"""
+    if t.dtype is not dtype or t.ndim != 1 or (count is not None and t.shape[0] != count):
+        raise ValueError(f"{name}: expected {dtype} [{'*' if count is None else count}], got {t.dtype} {tuple(t.shape)}")
+    return t.contiguous()
 
 
 def plan_kv_blocks(seq_lens: Tensor, new_tokens: Tensor, block_table: Tensor, free_blocks: Tensor,
@@ -98,29 +97,32 @@ def plan_kv_blocks(seq_lens: Tensor, new_tokens: Tensor, block_table: Tensor, fr
     slot is -1): a positive number of missing blocks, -1 for a request longer than its table
     row, -2 for more than `total_tokens` tokens, -3 for a free list that cannot be.  The
     inputs stay as they are; all tensors int32 on one GPU."""
-    lens = _int_tensor("seq_lens", seq_lens, torch.int32, None)
+    lens = _ints("seq_lens", seq_lens, torch.int32)
     requests = lens.shape[0]
-    add = _int_tensor("new_tokens", new_tokens, torch.int32, requests)
-    table = _int_tensor("block_table", block_table, torch.int32, requests, None)
-    free = _int_tensor("free_blocks", free_blocks, torch.int32, None)
-    count = _int_tensor("num_free", num_free, torch.int32, 1)
-    if total_tokens < 0 or block_size < 1 or table.shape[1] < 1:
-        raise ValueError(f"bad sizes: {total_tokens} tokens, blocks of {block_size}, {table.shape[1]} table columns")
-    device = _lib.require_gpu(lens, add, table, free, count)
-    lib = _lib.load()
-    with _lib.on_device(device):
-        # one allocation for the 32-bit outputs, cut at 16-byte boundaries
-        sizes = (requests, requests + 1, table.numel(), free.numel(), 1, 1)
-        padded = [-(-s // 4) * 4 for s in sizes]
-        lens_out, start, table_out, free_out, count_out, status = (
-            piece[:s] for piece, s in zip(torch.empty(sum(padded), dtype=torch.int32, device=device).split(padded), sizes))
-        slots = torch.empty(total_tokens, dtype=torch.int64, device=device)
-        _lib.check(lib.ctmi_kv_plan(
-            lens.data_ptr(), add.data_ptr(), table.data_ptr(), free.data_ptr(), count.data_ptr(), requests,
-            table.shape[1], free.shape[0], total_tokens, block_size, lens_out.data_ptr(), start.data_ptr(),
-            slots.data_ptr(), table_out.data_ptr(), free_out.data_ptr(), count_out.data_ptr(),
-            status.data_ptr(), _lib.stream_of(device)))
-    return KVPlan(lens_out, start, slots, table_out.view(table.shape), free_out, count_out, status)
+    add = _ints("new_tokens", new_tokens, torch.int32, requests)
+    free = _ints("free_blocks", free_blocks, torch.int32)
+    count = _ints("num_free", num_free, torch.int32, 1)
+    if block_table.dtype is not torch.int32 or block_table.ndim != 2 or block_table.shape[0] != requests:
+        raise ValueError(f"block_table: expected {torch.int32} [{requests}, *], got {block_table.dtype} {tuple(block_table.shape)}")
+    width, capacity = block_table.shape[1], free.shape[0]
+    if total_tokens < 0 or block_size < 1 or width < 1:
+        raise ValueError(f"bad sizes: {total_tokens} tokens, blocks of {block_size}, {width} table columns")
+    index = _lib.gpu_index(lens, add, block_table, free, count)
+    if not _lib.is_current(index):
+        with torch.cuda.device(index):
+            return plan_kv_blocks(lens, add, block_table, free, count, block_size=block_size, total_tokens=total_tokens)
+    table = block_table.contiguous()
+    # one allocation for the 32-bit outputs
+    lens_out, start, table_out, free_out, count_out, status = lens.new_empty(
+        2 * requests + requests * width + capacity + 3).split_with_sizes(
+            (requests, requests + 1, requests * width, capacity, 1, 1))
+    slots = torch.empty(total_tokens, dtype=torch.int64, device=lens.device)
+    _lib.check(_lib.load().ctmi_kv_plan(
+        lens.data_ptr(), add.data_ptr(), table.data_ptr(), free.data_ptr(), count.data_ptr(), requests, width,
+        capacity, total_tokens, block_size, lens_out.data_ptr(), start.data_ptr(), slots.data_ptr(),
+        table_out.data_ptr(), free_out.data_ptr(), count_out.data_ptr(), status.data_ptr(),
+        _lib.stream_of_index(index)))
+    return KVPlan(lens_out, start, slots, table_out.view(requests, width), free_out, count_out, status)
 
 
 def append_kv_blocks(key: Tensor, value: Tensor, blocks: KVBlocks, slots: Tensor, *, dynamic: bool = True) -> None:
@@ -143,19 +145,22 @@ def append_kv_blocks(key: Tensor, value: Tensor, blocks: KVBlocks, slots: Tensor
         raise NotImplementedError(f"keys and values must be bfloat16 or float16, got {key.dtype} and {value.dtype}")
     if torch.is_grad_enabled() and (key.requires_grad or value.requires_grad):
         raise NotImplementedError("append_kv_blocks has no backward: call it under torch.no_grad()")
-    slots = _int_tensor("slots", slots, torch.int64, key.shape[0])
-    device = _lib.require_gpu(key, value, slots, *blocks)
+    slots = _ints("slots", slots, torch.int64, key.shape[0])
+    index = _lib.gpu_index(key, value, slots, *blocks)
+    if not _lib.is_current(index):
+        with torch.cuda.device(index):
+            return append_kv_blocks(key, value, blocks, slots, dynamic=dynamic)
     key, value = _aligned(key), _aligned(value)
-    with _lib.on_device(device):
-        _lib.check(_lib.load().ctmi_kv_append(
-            key.data_ptr(), value.data_ptr(), _lib.dtype_code(key.dtype), key.stride(0), key.stride(1),
-            value.stride(0), value.stride(1), slots.data_ptr(), key.shape[0], ctypes.byref(c), int(dynamic),
-            _lib.stream_of(device)))
+    (kt, kh, _), (vt, vh, _) = key.stride(), value.stride()
+    _lib.check(_lib.load().ctmi_kv_append(
+        key.data_ptr(), value.data_ptr(), _lib.dtype_code(key.dtype), kt, kh, vt, vh, slots.data_ptr(), key.shape[0],
+        ctypes.byref(c), int(dynamic), _lib.stream_of_index(index)))
 
 
 def _aligned(t: Tensor) -> Tensor:
     """`t` [tokens, heads, dim], or a copy if its heads do not start at 16-byte boundaries"""
-    if t.stride(2) == 1 and t.stride(1) % 8 == 0 and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0:
+    token, head, inner = t.stride()
+    if inner == 1 and head % 8 == 0 and token % 8 == 0 and t.data_ptr() % 16 == 0:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -182,41 +187,44 @@ def attend_kv_blocks(query: Tensor, blocks: KVBlocks, block_table: Tensor, seq_l
         raise NotImplementedError(f"queries must be bfloat16 or float16, got {query.dtype}")
     if torch.is_grad_enabled() and query.requires_grad:
         raise NotImplementedError("attend_kv_blocks has no backward: call it under torch.no_grad()")
-    lens = _int_tensor("seq_lens", seq_lens, torch.int32, None)
+    lens = _ints("seq_lens", seq_lens, torch.int32)
     requests, (tokens, heads, dim) = lens.shape[0], query.shape
     if block_table.dtype is not torch.int32 or block_table.ndim != 2 or block_table.shape[0] != requests:
         raise ValueError(f"block_table: expected {torch.int32} [{requests}, *], got {block_table.dtype} {tuple(block_table.shape)}")
     width = block_table.shape[1]
-    if block_table.stride(1) != 1 or block_table.stride(0) < width:
-        block_table = block_table.contiguous()
     if query_start is not None:
-        query_start = _int_tensor("query_start", query_start, torch.int32, requests + 1)
+        query_start = _ints("query_start", query_start, torch.int32, requests + 1)
     elif tokens != requests:
         raise ValueError(f"without query_start every request has one token: got {tokens} tokens for {requests} requests")
-    if out is not None and (out.shape != query.shape or out.dtype is not query.dtype or not out.is_contiguous()
-                            or out.data_ptr() % 16):
-        raise ValueError(f"out: expected contiguous {query.dtype} {tuple(query.shape)}, 16-byte aligned")
-    device = _lib.require_gpu(query, block_table, lens, query_start, out, *blocks)
-    if out is not None and out.data_ptr() == query.data_ptr():
-        raise ValueError("out must not be the queries' memory")
+    if out is not None:
+        if out.shape != query.shape or out.dtype is not query.dtype or not out.is_contiguous() or out.data_ptr() % 16:
+            raise ValueError(f"out: expected contiguous {query.dtype} {tuple(query.shape)}, 16-byte aligned")
+        if out.untyped_storage().data_ptr() == query.untyped_storage().data_ptr():
+            raise ValueError("out must not share the queries' memory")
+    index = _lib.gpu_index(query, block_table, lens, query_start, out, *blocks)
+    if not _lib.is_current(index):
+        with torch.cuda.device(index):
+            return attend_kv_blocks(query, blocks, block_table, lens, query_start, max_query=max_query, max_seq=max_seq,
+                                    softmax_scale=softmax_scale, out=out)
+    table_stride, inner = block_table.stride()
+    if inner != 1 or table_stride < width:
+        block_table = block_table.contiguous()
+        table_stride = width
     query = _aligned(query)
-    if max_query is None:
-        max_query = 1 if query_start is None else tokens
-    if max_seq is None:
-        max_seq = width * c.block_size
-    max_query, max_seq = max(1, min(max_query, tokens)), max(1, min(max_seq, width * c.block_size))
+    longest = width * c.block_size
+    max_query = max(1, min(max_query, tokens)) if max_query is not None else 1 if query_start is None else max(1, tokens)
+    max_seq = max(1, longest if max_seq is None else min(max_seq, longest))
     scale = dim ** -0.5 if softmax_scale is None else float(softmax_scale)
     lib = _lib.load()
-    with _lib.on_device(device):
-        if out is None:
-            out = torch.empty((tokens, heads, dim), dtype=query.dtype, device=device)
-        tmp_bytes = lib.ctmi_kv_attend_tmp_bytes(tokens, requests, heads, c.kv_heads, dim, max_query, max_seq)
-        tmp = torch.empty(tmp_bytes, dtype=torch.uint8, device=device) if tmp_bytes else None
-        _lib.check(lib.ctmi_kv_attend(
-            query.data_ptr(), _lib.dtype_code(query.dtype), query.stride(0), query.stride(1), out.data_ptr(),
-            tokens, heads, ctypes.byref(c), block_table.data_ptr(), block_table.stride(0), width, lens.data_ptr(),
-            _lib.ptr(query_start), requests, scale, max_query, max_seq, _lib.ptr(tmp), tmp_bytes,
-            _lib.stream_of(device)))
+    if out is None:
+        out = query.new_empty((tokens, heads, dim))
+    tmp_bytes = lib.ctmi_kv_attend_tmp_bytes(tokens, requests, heads, c.kv_heads, dim, max_query, max_seq)
+    tmp = torch.empty(tmp_bytes, dtype=torch.uint8, device=out.device) if tmp_bytes else None
+    token_stride, head_stride, _ = query.stride()
+    _lib.check(lib.ctmi_kv_attend(
+        query.data_ptr(), _lib.dtype_code(query.dtype), token_stride, head_stride, out.data_ptr(), tokens, heads,
+        ctypes.byref(c), block_table.data_ptr(), table_stride, width, lens.data_ptr(), _lib.ptr(query_start), requests,
+        scale, max_query, max_seq, _lib.ptr(tmp), tmp_bytes, _lib.stream_of_index(index)))
     return out
 
 

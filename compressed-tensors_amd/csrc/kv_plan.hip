@@ -34,123 +34,131 @@ __device__ __forceinline__ int last_at_most(const int32_t* a, int n, int32_t v) 
   return lo;
 }
 
-// exclusive running sum of one number per thread over the workgroup; *total = the sum
-__device__ __forceinline__ int64_t scan256(int64_t v, int64_t* wave_sums, int64_t* total) {
+// exclusive running sums of two numbers per thread over the workgroup, in place; *all_ = the sums
+__device__ __forceinline__ void scan256(uint64_t& a, uint64_t& b, uint64_t (*sums)[2], uint64_t* all_a, uint64_t* all_b) {
   const int lane = lane_id(), wave = threadIdx.x / kWave;
-  int64_t up = v;
+  uint64_t up_a = a, up_b = b;
 #pragma unroll
   for (int d = 1; d < kWave; d *= 2) {
-    const int64_t o = __shfl_up(up, d, kWave);
-    if (lane >= d) up += o;
+    const uint64_t o_a = __shfl_up(up_a, d, kWave), o_b = __shfl_up(up_b, d, kWave);
+    if (lane >= d) up_a += o_a, up_b += o_b;
   }
-  __syncthreads();  // wave_sums may still be read from the call before
-  if (lane == kWave - 1) wave_sums[wave] = up;
+  if (lane == kWave - 1) sums[wave][0] = up_a, sums[wave][1] = up_b;
   __syncthreads();
-  int64_t before = 0, all = 0;
+  a = up_a - a, b = up_b - b;
+  *all_a = *all_b = 0;
 #pragma unroll
   for (int w = 0; w < kPlanThreads / kWave; ++w) {
-    if (w < wave) before += wave_sums[w];
-    all += wave_sums[w];
+    if (w < wave) a += sums[w][0], b += sums[w][1];
+    *all_a += sums[w][0], *all_b += sums[w][1];
   }
-  *total = all;
-  return before + up - v;
 }
+
+// A request in 32 bits: lengths are below 2^31, so is what a length and an addition need in
+// blocks, and every sum over the requests once they all fit their rows (requests x width is).
+struct PlanRequest {
+  uint32_t len, add, held, need;  // tokens, and blocks before and after
+  bool ends, fits;
+  __device__ __forceinline__ PlanRequest(const PlanArgs& a, int r) {
+    const int32_t l = a.lens[r], n = a.add[r];
+    const uint32_t bs = a.block_size;
+    len = (uint32_t)l, ends = n < 0, add = ends ? 0u : (uint32_t)n;
+    held = len / bs + (len % bs != 0);
+    const uint32_t after = len + add;
+    need = after / bs + (after % bs != 0);
+    fits = l >= 0 && need <= (uint32_t)a.width && held <= (uint32_t)a.width;
+  }
+};
 
 __global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(PlanArgs a) {
   extern __shared__ int32_t lds[];  // start, want, back: requests + 1 each
-  __shared__ int64_t wave_sums[kPlanThreads / kWave];
+  __shared__ uint64_t sums[kPlanThreads / kWave][2];
   const int n = a.requests;
   int32_t *start = lds, *want = lds + n + 1, *back = lds + 2 * (n + 1);
-  const int64_t bs = a.block_size;
+  const int32_t had = a.num_free[0];
 
   const int per = (n + kPlanThreads - 1) / kPlanThreads;
   const int r0 = min(n, (int)threadIdx.x * per), r1 = min(n, r0 + per);
-  int64_t tokens = 0, wants = 0, backs = 0;
-  int misfit = 0;
+  uint64_t tokens = 0, blocks = 0;  // blocks: those to take, and above 2^32 those that come back
+  bool misfit = false;
   for (int r = r0; r < r1; ++r) {
-    const int64_t len = a.lens[r], add = a.add[r];
-    const int64_t held = (len + bs - 1) / bs;
-    misfit |= len < 0 || held > a.width;
-    if (add < 0) {
-      backs += held;
-    } else {
-      const int64_t need = (len + add + bs - 1) / bs;
-      misfit |= need > a.width;
-      tokens += add;
-      wants += need - held;
-    }
+    const PlanRequest q(a, r);
+    misfit |= !q.fits;
+    tokens += q.add;
+    blocks += q.ends ? (uint64_t)q.held << 32 : (uint64_t)(q.need - q.held);
   }
+  uint64_t all_tokens, all_blocks;
+  scan256(tokens, blocks, sums, &all_tokens, &all_blocks);
   misfit = __syncthreads_or(misfit);
-  int64_t all_tokens, all_wants, all_backs;
-  int64_t t = scan256(tokens, wave_sums, &all_tokens);
-  int64_t w = scan256(wants, wave_sums, &all_wants);
-  int64_t b = scan256(backs, wave_sums, &all_backs);
+  const int64_t all_wants = (uint32_t)all_blocks, all_backs = all_blocks >> 32;
 
-  const int64_t had = a.num_free[0];
   int64_t status = 0;
   if (misfit) status = -1;
-  else if (all_tokens > a.slot_count) status = -2;
+  else if (all_tokens > (uint64_t)a.slot_count) status = -2;
   else if (had < 0 || had > a.capacity || had + all_backs > a.capacity) status = -3;
   else if (all_wants > had + all_backs) status = all_wants - had - all_backs;
   const bool ok = status == 0;
 
-  if (ok) {  // every sum fits 32 bits: tokens <= slot_count, blocks <= capacity
+  if (ok) {
+    uint32_t t = (uint32_t)tokens, w = (uint32_t)blocks, b = (uint32_t)(blocks >> 32);
     for (int r = r0; r < r1; ++r) {
-      const int64_t len = a.lens[r], add = a.add[r], held = (len + bs - 1) / bs;
+      const PlanRequest q(a, r);
       start[r] = (int32_t)t, want[r] = (int32_t)w, back[r] = (int32_t)b;
-      if (add < 0) b += held;
-      else t += add, w += (len + add + bs - 1) / bs - held;
+      t += q.add;
+      if (q.ends) b += q.held;
+      else w += q.need - q.held;
     }
     if (threadIdx.x == 0) start[n] = (int32_t)all_tokens, want[n] = (int32_t)all_wants, back[n] = (int32_t)all_backs;
   }
   __syncthreads();
 
-  const int64_t top = had + all_backs;  // height of the stack before the pops
+  const uint32_t width = (uint32_t)a.width;
+  const int32_t top = had + (int32_t)all_backs;  // height of the stack before the pops
   // entry p of the stack: the free list, above it what ended requests give back
-  auto stack = [&](int64_t p) -> int32_t {
+  auto stack = [&](int32_t p) -> int32_t {
     if (p < had) return a.free[p];
-    const int r = last_at_most(back, n, (int32_t)(p - had));
-    return a.table[(int64_t)r * a.width + (p - had - back[r])];
+    const int r = last_at_most(back, n, p - had);
+    return a.table[(uint32_t)r * width + (uint32_t)(p - had - back[r])];
   };
   // block `column` of request r, old or newly taken
-  auto block_of = [&](int r, int64_t column, int64_t held) -> int32_t {
-    return column < held ? a.table[(int64_t)r * a.width + column] : stack(top - 1 - (want[r] + column - held));
+  auto block_of = [&](int r, uint32_t column, uint32_t held) -> int32_t {
+    return column < held ? a.table[(uint32_t)r * width + column] : stack(top - 1 - (int32_t)((uint32_t)want[r] + column - held));
   };
 
-  const int64_t first = (int64_t)blockIdx.x * kPlanThreads + threadIdx.x, step = (int64_t)gridDim.x * kPlanThreads;
-  for (int64_t i = first; i < a.slot_count; i += step) {
+  const uint32_t first = blockIdx.x * kPlanThreads + threadIdx.x, step = gridDim.x * kPlanThreads;
+  for (uint32_t i = first; i < (uint32_t)a.slot_count; i += step) {
     int64_t slot = -1;
     if (ok && i < all_tokens) {
       const int r = last_at_most(start, n, (int32_t)i);
-      const int64_t len = a.lens[r], place = len + (i - start[r]);
-      const int64_t block = block_of(r, place / bs, (len + bs - 1) / bs);
-      if (block >= 0) slot = block * bs + place % bs;
+      const PlanRequest q(a, r);
+      const uint32_t place = q.len + (i - (uint32_t)start[r]), bs = a.block_size, column = place / bs;
+      const int64_t block = block_of(r, column, q.held);
+      if (block >= 0) slot = block * bs + (place - column * bs);
     }
     a.slots[i] = slot;
   }
-  for (int64_t i = first; i < (int64_t)n * a.width; i += step) {
-    const int r = (int)(i / a.width);
-    const int64_t column = i - (int64_t)r * a.width;
+  for (uint32_t i = first; i < (uint32_t)n * width; i += step) {
     int32_t v = a.table[i];
     if (ok) {
-      const int64_t len = a.lens[r], add = a.add[r], held = (len + bs - 1) / bs;
-      if (add < 0) v = -1;
-      else if (column >= held && column < (len + add + bs - 1) / bs) v = block_of(r, column, held);
+      const uint32_t r = i / width, column = i - r * width;
+      const PlanRequest q(a, (int)r);
+      if (q.ends) v = -1;
+      else if (column >= q.held && column < q.need) v = block_of((int)r, column, q.held);
     }
     a.table_out[i] = v;
   }
-  const int64_t left = ok ? top - all_wants : had;
-  for (int64_t i = first; i < a.capacity; i += step)
-    a.free_out[i] = !ok ? a.free[i] : i < left ? stack(i) : -1;
-  for (int64_t i = first; i <= n; i += step) {
+  const int32_t left = ok ? top - (int32_t)all_wants : had;
+  for (uint32_t i = first; i < (uint32_t)a.capacity; i += step)
+    a.free_out[i] = !ok ? a.free[i] : (int32_t)i < left ? stack((int32_t)i) : -1;
+  for (uint32_t i = first; i <= (uint32_t)n; i += step) {
     a.start[i] = ok ? start[i] : 0;
-    if (i < n) {
+    if (i < (uint32_t)n) {
       const int32_t len = a.lens[i], add = a.add[i];
       a.lens_out[i] = !ok ? len : add < 0 ? 0 : len + add;
     }
   }
   if (first == 0) {
-    a.num_free_out[0] = (int32_t)left;
+    a.num_free_out[0] = left;
     a.status[0] = (int32_t)status;
   }
 }
@@ -171,8 +179,9 @@ extern "C" int ctmi_kv_plan(const int32_t* seq_lens, const int32_t* new_tokens, 
                (long long)requests, (long long)width, (long long)free_capacity, (long long)slot_count);
   CTMI_REQUIRE(requests <= kPlanMaxRequests, CTMI_ERR_UNSUPPORTED, "at most %lld requests per call, got %lld",
                (long long)kPlanMaxRequests, (long long)requests);
-  CTMI_REQUIRE(width < (1ll << 31) && free_capacity < (1ll << 31) && slot_count < (1ll << 31), CTMI_ERR_UNSUPPORTED,
-               "table columns, free blocks and slots must each stay below 2^31");
+  CTMI_REQUIRE(width < (1ll << 31) && (requests == 0 || width < (1ll << 31) / requests) &&
+                   free_capacity < (1ll << 31) && slot_count < (1ll << 31),
+               CTMI_ERR_UNSUPPORTED, "table entries, free blocks and slots must each stay below 2^31");
   CTMI_REQUIRE(block_size >= 1, CTMI_ERR_VALUE, "block_size must be at least 1, got %d", block_size);
   CTMI_REQUIRE(num_free && query_start && num_free_out && status &&
                    (requests == 0 || (seq_lens && new_tokens && block_table && seq_lens_out && table_out)) &&
