@@ -43,7 +43,6 @@ struct LinearArgs {
   float* part;  // [split][m][n], or NULL
   int32_t m, n, k, group, groups, words;
   int32_t wave_k;  // columns a wavefront takes
-  int32_t pair_groups, pair_rest;  // 256 columns = pair_groups groups and pair_rest columns
 };
 
 struct Operand {
@@ -121,56 +120,59 @@ struct Buffer {
 };
 
 // SMALL: groups that are no multiple of 128 columns, so a scale holds for one product of 32
-// columns only.  WIDE: scales are fp32, else of x's type.
+// columns only.  WIDE: scales are fp32, else of x's type.  XL: loads of 4 rows of x each, as
+// many as there are rows (one for a decoding request or four).
 //
 // A wavefront keeps two steps requested: a slot is loaded again as soon as its step is
 // multiplied.  The slots are registers by name, the loads stand in no branch (behind the last
-// step they read nothing) and rows behind the last are read as the last (their sums are
-// dropped): a load that may not have been issued, or a copy of a register that is still to
-// arrive, would make the wait for one step a wait for all.  The loop holds the two steps and
-// nothing is unrolled beyond them: a wavefront runs few steps, and code it has to fetch for
-// each of them costs more than the steps do.
-template <typename T, int MT, int NT, bool SMALL, bool WIDE>
+// step they read nothing): a load that may not have been issued, or a copy of a register that
+// is still to arrive, would make the wait for one step a wait for all.  The loop holds the two
+// steps and nothing is unrolled beyond them: a wavefront runs few steps, and code it has to
+// fetch for each of them costs more than the steps do.
+//
+// What a compute unit's loads cost is the places they touch: lanes next to each other in one
+// line are looked up together, others one by one.  So x comes in rows of 256 bytes, 16 lanes
+// each, and reaches the operands' layout through the wavefront's own 4 KB of LDS per 16 rows
+// (pieces of a row swapped by the row's number: no bank is hit twice); and one load brings the
+// scales of all NT x 16 weight rows, one lane each, from where the lanes that use them take
+// them.  With operands loaded where they are used, 16 x 28672 x 4096 took 26 us, 7 of them for
+// x and 4 for scales.
+template <typename T, int MT, int NT, int XL, bool SMALL, bool WIDE>
 struct LinearWave {
+  static constexpr int PARTS = SMALL ? 4 : 1;  // groups in a step
   struct Step {
     Vec<uint32_t, 4> w[NT];
-    Vec<uint32_t, 4> x[MT][4];
-  };
-  // as loaded, for a pair of steps, a different group in each lane group.  SMALL: entry i is
-  // step i, lane group j its columns 32 j ... 32 j + 31; otherwise lane group j is step j % 2.
-  static constexpr int RAW = SMALL ? 2 : 1;
-  struct Scales {
-    uint32_t s[RAW][NT], z[RAW][NT];
+    uint32_t s[PARTS], z[PARTS];  // scale of weight row `lane`, zero points of rows 8 (lane % 8) on
+    Vec<uint32_t, 4> x[XL];       // rows 4 i + lane / 16, columns (lane % 16) * 8 on
   };
 
   const LinearArgs& a;
-  int c, j;
+  int lane, c, j;
   // where there are no zero points the buffer is empty, reads 0, and every zero point is 8
   uint32_t z_none;
-  Buffer w_buf, s_buf, z_buf, x_buf;  // of the workgroup's rows
-  uint32_t w_at[NT], s_at[NT], z_at[NT], x_at[MT];
+  Buffer w_buf, s_buf, z_buf, x_buf;  // of the workgroup's rows; rows behind the last read as 0
+  uint32_t w_at, s_at, z_at, x_at, w_tile, x_four;
+  Vec<uint32_t, 4>* mine;  // of LDS
   f32x4 y[NT][MT];
 
-  __device__ __forceinline__ LinearWave(const LinearArgs& args, int n0, int m0)
+  __device__ __forceinline__ LinearWave(const LinearArgs& args, int n0, int m0, Vec<uint32_t, 4>* lds)
       : a(args),
         w_buf(a.packed + (int64_t)n0 * a.words, (uint32_t)min(NT * 16, a.n - n0) * (uint32_t)a.words * 4u),
         s_buf((const uint8_t*)a.scale + (int64_t)n0 * a.groups * (WIDE ? 4 : 2),
               (uint32_t)min(NT * 16, a.n - n0) * (uint32_t)a.groups * (WIDE ? 4 : 2)),
         z_buf(a.zero + (int64_t)(n0 >> 3) * a.groups, a.zero ? (uint32_t)((min(NT * 16, a.n - n0) + 7) >> 3) * (uint32_t)a.groups * 4u : 0u),
-        x_buf(a.x + m0 * a.x_stride, ((uint32_t)(min(MT * 16, a.m - m0) - 1) * (uint32_t)a.x_stride + (uint32_t)a.k) * 2u) {
-    const int lane = lane_id();
-    c = lane & 15, j = lane >> 4;
+        x_buf(a.x + m0 * a.x_stride, ((uint32_t)(min(MT * 16, a.m - m0) - 1) * (uint32_t)a.x_stride + (uint32_t)a.k) * 2u),
+        mine(lds) {
+    lane = lane_id(), c = lane & 15, j = lane >> 4;
     z_none = a.zero ? 0u : 8u;
+    w_at = (uint32_t)c * (uint32_t)a.words * 4u + j * 16;
+    w_tile = (uint32_t)a.words * 64u;
+    s_at = (uint32_t)(lane % (NT * 16)) * (uint32_t)a.groups * (WIDE ? 4 : 2);  // n0 is a multiple of 16
+    z_at = (uint32_t)(lane & 7) * (uint32_t)a.groups * 4u;
+    x_at = (uint32_t)j * (uint32_t)a.x_stride * 2u + c * 16;
+    x_four = (uint32_t)a.x_stride * 8u;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const int row = min(t * 16 + c, a.n - 1 - n0);  // n0 is a multiple of 16
-      w_at[t] = (uint32_t)row * (uint32_t)a.words * 4u + j * 16;
-      s_at[t] = (uint32_t)row * (uint32_t)a.groups * (WIDE ? 4 : 2);
-      z_at[t] = (uint32_t)(row >> 3) * (uint32_t)a.groups * 4u;
-    }
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-      x_at[mt] = (uint32_t)min(mt * 16 + c, a.m - 1 - m0) * (uint32_t)a.x_stride * 2u + j * 16;
+    for (int i = XL; i < MT * 4; ++i) mine[i * 64 + lane] = Vec<uint32_t, 4>{};
     clear();
   }
 
@@ -181,43 +183,34 @@ struct LinearWave {
       for (int mt = 0; mt < MT; ++mt) y[t][mt] = f32x4{0, 0, 0, 0};
   }
 
-  // the group of this lane's columns in pairs of steps as they are loaded, one after the other
+  // the group of the next columns, and how many of it are left, as steps are loaded one after
+  // the other
   struct Groups {
-    int g[RAW], left[RAW];  // and how many columns of it follow
+    int g, left;
   };
   __device__ __forceinline__ Groups groups_at(int kb) const {
-    Groups at;
-#pragma unroll
-    for (int i = 0; i < RAW; ++i) {
-      const int k = kb + (SMALL ? i * kStepK + j * 32 : (j & 1) * kStepK);
-      at.g[i] = k / a.group, at.left[i] = (at.g[i] + 1) * a.group - k;
-    }
-    return at;
+    const int g = kb / a.group;
+    return Groups{g, (g + 1) * a.group - kb};
   }
-  __device__ __forceinline__ void load_scales(Scales& sc, Groups& at) const {
+  __device__ __forceinline__ void load_scales(Step& st, Groups& at, bool there) const {
 #pragma unroll
-    for (int i = 0; i < RAW; ++i) {
-      const uint32_t g = min(at.g[i], a.groups - 1);
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        sc.s[i][t] = WIDE ? s_buf.load4(s_at[t] + g * 4u) : s_buf.load2(s_at[t] + g * 2u);
-        sc.z[i][t] = z_buf.load4(z_at[t] + g * 4u);
-      }
-      at.g[i] += a.pair_groups, at.left[i] -= a.pair_rest;
-      if (at.left[i] <= 0) at.left[i] += a.group, ++at.g[i];
+    for (int i = 0; i < PARTS; ++i) {
+      const uint32_t g = min(at.g, a.groups - 1);
+      st.s[i] = WIDE ? s_buf.load4(there ? s_at + g * 4u : kNowhere) : s_buf.load2(there ? s_at + g * 2u : kNowhere);
+      st.z[i] = z_buf.load4(there ? z_at + g * 4u : kNowhere);
+      at.left -= SMALL ? 32 : kStepK;
+      const int over = (int)((uint32_t)(at.left - 1) >> 31);  // no branch here either
+      at.left += -over & a.group, at.g += over;
     }
   }
-  __device__ __forceinline__ float scale_of(uint32_t raw) const { return WIDE ? u2f(raw) : T::to_f32((uint16_t)raw); }
-  __device__ __forceinline__ float zero_of(uint32_t raw) const { return (float)(((raw >> (4 * (c & 7))) & 15u) | z_none); }
 
-  __device__ __forceinline__ void load(Step& st, int kb, bool there) const {
-    const uint32_t wk = there ? (uint32_t)kb / 2u : kNowhere, xk = there ? (uint32_t)kb * 2u : kNowhere;
+  __device__ __forceinline__ void load(Step& st, int kb, bool there, Groups& at) const {
+    const uint32_t wk = there ? w_at + (uint32_t)kb / 2u : kNowhere, xk = there ? x_at + (uint32_t)kb * 2u : kNowhere;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) st.w[t] = w_buf.load16(w_at[t] + wk);
+    for (int t = 0; t < NT; ++t) st.w[t] = w_buf.load16(wk + t * w_tile);
+    load_scales(st, at, there);
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int t = 0; t < 4; ++t) st.x[mt][t] = x_buf.load16(x_at[mt] + xk + t * 64);
+    for (int i = 0; i < XL; ++i) st.x[i] = x_buf.load16(xk + i * x_four);
   }
 
   // a step that may end behind the row, or of rows that do not start at 16-byte boundaries
@@ -226,75 +219,84 @@ struct LinearWave {
     for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        st.w[t].v[i] = w_buf.load4(kb / 8 + j * 4 + i < a.words ? w_at[t] + kb / 2 + i * 4 : kNowhere);
+        st.w[t].v[i] = w_buf.load4(kb / 8 + j * 4 + i < a.words ? w_at + kb / 2 + t * w_tile + i * 4 : kNowhere);
+    Groups at = groups_at(kb);
+    load_scales(st, at, true);
+#pragma unroll
+    for (int i = 0; i < XL; ++i) {
+      const int first = kb + c * 8;
+      const uint32_t at = x_at + kb * 2 + i * x_four;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        st.x[i].v[e] = x_buf.load2(first + 2 * e < a.k ? at + 4 * e : kNowhere) |
+                       x_buf.load2(first + 2 * e + 1 < a.k ? at + 4 * e + 2 : kNowhere) << 16;
+    }
+  }
+
+  template <bool SIGNED>
+  __device__ __forceinline__ void step(Step& st) {
+    const Operand ones = T::id == CTMI_BF16 ? Operand{{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u}}
+                                            : Operand{{0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u}};
+#pragma unroll
+    for (int i = 0; i < XL; ++i) mine[(i * 4 + j) * 16 + (c ^ ((i * 4 + j) & 15))] = st.x[i];
+    Operand x[MT][4];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const int first = kb + t * 32 + j * 8;
-        const uint32_t at = x_at[mt] + kb * 2 + t * 64;
+      for (int t = 0; t < 4; ++t) x[mt][t] = __builtin_bit_cast(Operand, mine[(mt * 16 + c) * 16 + ((t * 4 + j) ^ c)]);
+    auto add = [&](f32x4 sum, const Operand& v) { return product<T>(v, ones, sum); };
+    auto scale_zero = [&](int nt, int part, float& s, float& z) {
+      const uint32_t raw = __shfl(st.s[part], nt * 16 + c, kWave), zeros = __shfl(st.z[part], nt * 2 + (c >> 3), kWave);
+      s = WIDE ? u2f(raw) : T::to_f32((uint16_t)raw);
+      z = (float)(((zeros >> (4 * (c & 7))) & 15u) | z_none);
+    };
+    auto take = [&](int nt, int mt, float s, float z, const f32x4& acc, const f32x4& sum) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          st.x[mt][t].v[e] = x_buf.load2(first + 2 * e < a.k ? at + 4 * e : kNowhere) |
-                             x_buf.load2(first + 2 * e + 1 < a.k ? at + 4 * e + 2 : kNowhere) << 16;
+      for (int i = 0; i < 4; ++i) y[nt][mt][i] = fmaf(s, SIGNED ? acc[i] : fmaf(-z, sum[i], acc[i]), y[nt][mt][i]);
+    };
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) transpose4(st.w[nt].v);
+    f32x4 sums[MT];
+    if constexpr (SMALL) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) sums[mt] = add(f32x4{0, 0, 0, 0}, x[mt][t]);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float s, z;
+          scale_zero(nt, t, s, z);
+          const Operand w = SIGNED ? signed_codes_of<T>(st.w[nt].v[t], z) : codes_of<T>(st.w[nt].v[t]);
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) take(nt, mt, s, z, product<T>(x[mt][t], w, f32x4{0, 0, 0, 0}), sums[mt]);
+        }
+        // (the scales of all parts and tiles together would not leave registers for the rest)
+        __builtin_amdgcn_sched_barrier(0);
       }
-  }
-
-  // s, z: scale and zero point of each tile's column and, SMALL, of this lane's 32 columns
-  template <bool SIGNED>
-  __device__ __forceinline__ void step(Step& st, const float* scales, const float* zeros) {
-    const Operand ones = T::id == CTMI_BF16 ? Operand{{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u}}
-                                            : Operand{{0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u}};
-    constexpr int PARTS = SMALL ? 4 : 1;
-    f32x4 sums[PARTS][MT];
-    if constexpr (!SIGNED) {
+    } else {
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
+        sums[mt] = f32x4{0, 0, 0, 0};
 #pragma unroll
-        for (int i = 0; i < PARTS; ++i) sums[i][mt] = f32x4{0, 0, 0, 0};
+        for (int t = 0; t < 4; ++t) sums[mt] = add(sums[mt], x[mt][t]);
+      }
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
-          sums[SMALL ? t : 0][mt] = product<T>(__builtin_bit_cast(Operand, st.x[mt][t]), ones, sums[SMALL ? t : 0][mt]);
+      for (int nt = 0; nt < NT; ++nt) {
+        float s, z;
+        scale_zero(nt, 0, s, z);
+        f32x4 acc[MT];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) acc[mt] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const Operand w = SIGNED ? signed_codes_of<T>(st.w[nt].v[t], z) : codes_of<T>(st.w[nt].v[t]);
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) acc[mt] = product<T>(x[mt][t], w, acc[mt]);
+        }
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) take(nt, mt, s, z, acc[mt], sums[mt]);
       }
     }
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      transpose4(st.w[nt].v);
-      float s = scales[nt], z = zeros[nt];
-      f32x4 acc[MT];
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        if constexpr (SMALL) s = __shfl(scales[nt], t * 16 + c, kWave), z = __shfl(zeros[nt], t * 16 + c, kWave);
-        const Operand w = SIGNED ? signed_codes_of<T>(st.w[nt].v[t], z) : codes_of<T>(st.w[nt].v[t]);
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          if (t == 0 || SMALL) acc[mt] = f32x4{0, 0, 0, 0};
-          acc[mt] = product<T>(__builtin_bit_cast(Operand, st.x[mt][t]), w, acc[mt]);
-          if (SMALL || t == 3) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float v = SIGNED ? acc[mt][i] : fmaf(-z, sums[SMALL ? t : 0][mt][i], acc[mt][i]);
-              y[nt][mt][i] = fmaf(s, v, y[nt][mt][i]);
-            }
-          }
-        }
-      }
-    }
-  }
-
-  // the scales of a pair's steps, in the lanes that use them
-  __device__ __forceinline__ void spread(const Scales& raw, float (*s)[NT], float (*z)[NT]) const {
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        if constexpr (SMALL) {
-          s[i][t] = scale_of(raw.s[i][t]), z[i][t] = zero_of(raw.z[i][t]);
-        } else {
-          s[i][t] = __shfl(scale_of(raw.s[0][t]), i * 16 + c, kWave);
-          z[i][t] = __shfl(zero_of(raw.z[0][t]), i * 16 + c, kWave);
-        }
-      }
   }
 
   // columns k0 ... k1 - 1; those behind the last whole step (all of them, if the rows of the
@@ -304,21 +306,16 @@ struct LinearWave {
     const int end = aligned ? k0 + (min(k1, a.k) - k0) / kStepK * kStepK : k0;
     if (k0 < end) {
       Step one, two;
-      Scales raw;
       Groups at = groups_at(k0);
-      load_scales(raw, at);
-      load(one, k0, true);
-      load(two, k0 + kStepK, k0 + kStepK < end);
+      load(one, k0, true, at);
+      load(two, k0 + kStepK, k0 + kStepK < end, at);
 #pragma unroll 1
       for (int kb = k0; kb < end; kb += 2 * kStepK) {
-        float s[2][NT], z[2][NT];
-        spread(raw, s, z);
-        load_scales(raw, at);
-        step<false>(one, s[0], z[0]);
-        load(one, kb + 2 * kStepK, kb + 2 * kStepK < end);
+        step<false>(one);
+        load(one, kb + 2 * kStepK, kb + 2 * kStepK < end, at);
         __builtin_amdgcn_sched_barrier(0);
-        step<false>(two, s[1], z[1]);
-        load(two, kb + 3 * kStepK, kb + 3 * kStepK < end);
+        step<false>(two);
+        load(two, kb + 3 * kStepK, kb + 3 * kStepK < end, at);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
@@ -329,24 +326,21 @@ struct LinearWave {
 #pragma unroll 1
     for (int kb = k0; kb < k1; kb += kStepK) {
       Step st;
-      Scales raw;
-      Groups at = groups_at(kb);
-      float s[2][NT], z[2][NT];
       load_guarded(st, kb);
-      load_scales(raw, at);
-      spread(raw, s, z);
-      step<true>(st, s[0], z[0]);
+      step<true>(st);
     }
   }
 };
 
-template <typename T, int MT, int NT, bool SMALL, bool WIDE, int WAVES, int PER_SIMD>
+template <typename T, int MT, int NT, int XL, bool SMALL, bool WIDE, int WAVES, int PER_SIMD>
 __global__ __launch_bounds__(WAVES* kWave, PER_SIMD) void packed_linear_kernel(LinearArgs a) {
   constexpr int TM = MT * 16, TN = NT * 16;
-  extern __shared__ float meet[];  // [wave][TM][TN]
+  // each wavefront's x, TM rows of 256 bytes; at the end [wave][TM][TN] sums
+  extern __shared__ Vec<uint32_t, 4> lds[];
+  float* meet = (float*)lds;
   const int wave = threadIdx.x / kWave, waves = blockDim.x / kWave;
   const int n0 = blockIdx.x * TN;
-  LinearWave<T, MT, NT, SMALL, WIDE> w(a, n0, blockIdx.y * TM);
+  LinearWave<T, MT, NT, XL, SMALL, WIDE> w(a, n0, blockIdx.y * TM, lds + wave * TM * 16);
   const int64_t begin = ((int64_t)blockIdx.z * waves + wave) * a.wave_k;
   const int k0 = (int)(begin < a.k ? begin : a.k), k1 = (int)(begin + a.wave_k < a.k ? begin + a.wave_k : a.k);
   int redo = w.run((int)k0, k1);
@@ -359,6 +353,7 @@ __global__ __launch_bounds__(WAVES* kWave, PER_SIMD) void packed_linear_kernel(L
       for (int i = 0; i < 4; ++i) bad |= !(fabsf(w.y[nt][mt][i]) <= 3.4028235e38f);
   if (__any(bad)) w.clear(), redo = (int)k0;
   w.run_signed(redo, k1);
+  __syncthreads();  // sums take the place of x
   const int m0 = blockIdx.y * TM, rows = min(TM, a.m - m0);
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
@@ -409,7 +404,7 @@ LinearLaunch plan_linear(int64_t m, int64_t n, int64_t k) {
     l.nt = l.mt == 4 ? 2 : 4;
     l.waves = 4;
     const int64_t units = cdiv(tiles, l.nt) * m_blocks;
-    while (units * l.splits < 256 && k / (l.waves * l.splits * 2) >= 256 && l.splits < 16) l.splits *= 2;
+    while (units * l.splits < 512 && k / (l.waves * l.splits * 2) >= 256 && l.splits < 16) l.splits *= 2;
   }
   l.wave_k = cdiv(cdiv(k, l.waves * l.splits), kStepK) * kStepK;
   return l;
@@ -456,29 +451,34 @@ extern "C" int ctmi_packed_linear(const void* x, int32_t x_dtype, int64_t x_stri
   CTMI_REQUIRE(cdiv(m, tm) < (1 << 16), CTMI_ERR_UNSUPPORTED, "too many rows: %lld", (long long)m);
   LinearArgs a{(const uint16_t*)x, x_stride, (const uint32_t*)packed, scale, (const uint32_t*)zero_point,
                (const uint16_t*)bias, (uint16_t*)out, need ? (float*)tmp : nullptr, (int32_t)m, (int32_t)n,
-               (int32_t)k, (int32_t)group, (int32_t)(k / group), (int32_t)cdiv(k, 8), (int32_t)l.wave_k,
-               (int32_t)(2 * kStepK / group), (int32_t)(2 * kStepK % group)};
+               (int32_t)k, (int32_t)group, (int32_t)(k / group), (int32_t)cdiv(k, 8), (int32_t)l.wave_k};
   const dim3 grid((unsigned)cdiv(n, tn), (unsigned)cdiv(m, tm), (unsigned)l.splits), threads(l.waves * kWave);
-  const size_t lds = (size_t)l.waves * tm * tn * sizeof(float);
+  const size_t lds = (size_t)l.waves * tm * (tn * 4 > 256 ? tn * 4 : 256);
   const hipStream_t s = (hipStream_t)stream;
   const bool small = group % kStepK != 0 && group != k;
-#define LAUNCH(T, MT, NT, W, P)                                                                       \
+#define LAUNCH(T, MT, NT, XL, W, P)                                                                   \
   do {                                                                                                \
     if (scale_dtype == CTMI_F32) {                                                                    \
-      if (small) packed_linear_kernel<T, MT, NT, true, true, W, P><<<grid, threads, lds, s>>>(a);     \
-      else packed_linear_kernel<T, MT, NT, false, true, W, P><<<grid, threads, lds, s>>>(a);          \
+      if (small) packed_linear_kernel<T, MT, NT, XL, true, true, W, P><<<grid, threads, lds, s>>>(a);  \
+      else packed_linear_kernel<T, MT, NT, XL, false, true, W, P><<<grid, threads, lds, s>>>(a);       \
     } else {                                                                                          \
-      if (small) packed_linear_kernel<T, MT, NT, true, false, W, P><<<grid, threads, lds, s>>>(a);    \
-      else packed_linear_kernel<T, MT, NT, false, false, W, P><<<grid, threads, lds, s>>>(a);         \
+      if (small) packed_linear_kernel<T, MT, NT, XL, true, false, W, P><<<grid, threads, lds, s>>>(a); \
+      else packed_linear_kernel<T, MT, NT, XL, false, false, W, P><<<grid, threads, lds, s>>>(a);      \
     }                                                                                                 \
   } while (0)
 #define BY_SIZE(T)                                  \
   do {                                              \
-    if (l.mt == 4) LAUNCH(T, 4, 2, 4, 2);           \
-    else if (l.mt == 2) LAUNCH(T, 2, 4, 4, 2);      \
-    else if (l.nt == 4) LAUNCH(T, 1, 4, 4, 3);      \
-    else if (l.nt == 2) LAUNCH(T, 1, 2, 8, 4);      \
-    else LAUNCH(T, 1, 1, 8, 4);                     \
+    if (l.mt == 4) LAUNCH(T, 4, 2, 16, 4, 2);       \
+    else if (l.mt == 2) LAUNCH(T, 2, 4, 8, 4, 2);   \
+    else if (m > 4) {                               \
+      if (l.nt == 4) LAUNCH(T, 1, 4, 4, 4, 3);      \
+      else if (l.nt == 2) LAUNCH(T, 1, 2, 4, 8, 4); \
+      else LAUNCH(T, 1, 1, 4, 8, 4);                \
+    } else {                                        \
+      if (l.nt == 4) LAUNCH(T, 1, 4, 1, 4, 4);      \
+      else if (l.nt == 2) LAUNCH(T, 1, 2, 1, 8, 4); \
+      else LAUNCH(T, 1, 1, 1, 8, 4);                \
+    }                                               \
     if (need) packed_linear_join_kernel<T><<<dim3((unsigned)(cdiv(m * n, 256) < 2048 ? cdiv(m * n, 256) : 2048)), dim3(256), 0, s>>>(a, (int)l.splits); \
   } while (0)
   if (x_dtype == CTMI_BF16) BY_SIZE(BF16);
