@@ -70,6 +70,8 @@ def packed_linear(x: Tensor, weight_packed: Tensor, weight_scale: Tensor,
     weight_packed, weight_scale = weight_packed.contiguous(), weight_scale.contiguous()
     rows = x if x.ndim == 2 else x.reshape(-1, k)
     m, (stride, inner) = rows.shape[0], rows.stride()
+    if m > 16 and weight_packed.data_ptr() % 16:
+        weight_packed = weight_packed.clone()
     # rows that start at 16-byte boundaries are read in place
     if inner != 1 or stride % 8 or rows.data_ptr() % 16 or (m > 1 and not k <= stride < 1 << 24):
         rows = x.new_empty((m, (k + 7) // 8 * 8))[:, :k].copy_(rows)

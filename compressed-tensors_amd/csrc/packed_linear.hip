@@ -42,7 +42,8 @@ struct LinearArgs {
   uint16_t* out;
   float* part;  // [split][m][n], or NULL
   int32_t m, n, k, group, groups, words;
-  int32_t wave_k;  // columns a wavefront takes
+  int32_t wave_k;   // columns a wavefront takes
+  int32_t aligned;  // whole 8s of columns, weight rows at 16-byte boundaries
 };
 
 struct Operand {
@@ -205,7 +206,8 @@ struct LinearWave {
   }
 
   __device__ __forceinline__ void load(Step& st, int kb, bool there, Groups& at) const {
-    const uint32_t wk = there ? w_at + (uint32_t)kb / 2u : kNowhere, xk = there ? x_at + (uint32_t)kb * 2u : kNowhere;
+    // (behind the row's end x is 0 and the codes are the next row's: they do not count)
+    const uint32_t wk = there ? w_at + (uint32_t)kb / 2u : kNowhere, xk = (int)there & (int)(kb + c * 8 < a.k) ? x_at + (uint32_t)kb * 2u : kNowhere;
 #pragma unroll
     for (int t = 0; t < NT; ++t) st.w[t] = w_buf.load16(wk + t * w_tile);
     load_scales(st, at, there);
@@ -213,7 +215,7 @@ struct LinearWave {
     for (int i = 0; i < XL; ++i) st.x[i] = x_buf.load16(xk + i * x_four);
   }
 
-  // a step that may end behind the row, or of rows that do not start at 16-byte boundaries
+  // a step of rows that need not start at 16-byte boundaries, element by element
   __device__ __forceinline__ void load_guarded(Step& st, int kb) const {
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -299,11 +301,10 @@ struct LinearWave {
     }
   }
 
-  // columns k0 ... k1 - 1; those behind the last whole step (all of them, if the rows of the
-  // weight do not start at 16-byte boundaries) are left to run_signed
+  // columns k0 ... k1 - 1; returns where it stopped: nothing is done, and all left to
+  // run_signed, if the rows of the weight do not start at 16-byte boundaries
   __device__ __forceinline__ int run(int k0, int k1) {
-    const bool aligned = a.words % 4 == 0 && ((uintptr_t)a.packed & 15) == 0;
-    const int end = aligned ? k0 + (min(k1, a.k) - k0) / kStepK * kStepK : k0;
+    const int end = a.aligned ? k1 : k0;
     if (k0 < end) {
       Step one, two;
       Groups at = groups_at(k0);
@@ -377,6 +378,223 @@ __global__ __launch_bounds__(WAVES* kWave, PER_SIMD) void packed_linear_kernel(L
   }
 }
 
+// More than 16 rows: 8 wavefronts, 4 beside each other along n (NT tiles each) and 2 along k.
+// A compute unit then needs each element of x once: the 4 load a step of it together, two steps
+// ahead, into LDS.  (Each wavefront with x of its own, which is 4 times as much from the second
+// level cache, took 34 us for 64 x 4096 x 14336.)
+template <typename T, int MT, int NT, bool SMALL, bool WIDE>
+struct LinearShared {
+  static constexpr int PARTS = SMALL ? 4 : 1, ACROSS = 4, ALONG = 2;
+  struct Step {
+    Vec<uint32_t, 4> w[NT];
+    uint32_t s[PARTS], z[PARTS];
+  };
+  const LinearArgs& a;
+  int lane, c, j;
+  uint32_t z_none;
+  Buffer w_buf, s_buf, z_buf, x_buf;
+  uint32_t w_at, s_at, z_at, x_at, w_tile, x_four;
+  int across;
+  f32x4 y[NT][MT];
+
+  // n0: the wavefront's first column; one behind the last has empty buffers
+  __device__ __forceinline__ LinearShared(const LinearArgs& args, int n0, int m0, int wn)
+      : a(args),
+        w_buf(a.packed + (int64_t)min(n0, a.n - 1) * a.words, (uint32_t)max(min(NT * 16, a.n - n0), 0) * (uint32_t)a.words * 4u),
+        s_buf((const uint8_t*)a.scale + (int64_t)min(n0, a.n - 1) * a.groups * (WIDE ? 4 : 2),
+              (uint32_t)max(min(NT * 16, a.n - n0), 0) * (uint32_t)a.groups * (WIDE ? 4 : 2)),
+        z_buf(a.zero + (int64_t)(min(n0, a.n - 1) >> 3) * a.groups,
+              a.zero ? (uint32_t)((max(min(NT * 16, a.n - n0), 0) + 7) >> 3) * (uint32_t)a.groups * 4u : 0u),
+        x_buf(a.x + m0 * a.x_stride, ((uint32_t)(min(MT * 16, a.m - m0) - 1) * (uint32_t)a.x_stride + (uint32_t)a.k) * 2u),
+        across(wn) {
+    lane = lane_id(), c = lane & 15, j = lane >> 4;
+    z_none = a.zero ? 0u : 8u;
+    w_at = (uint32_t)c * (uint32_t)a.words * 4u + j * 16;
+    w_tile = (uint32_t)a.words * 64u;
+    s_at = (uint32_t)(lane % (NT * 16)) * (uint32_t)a.groups * (WIDE ? 4 : 2);
+    z_at = (uint32_t)(lane & 7) * (uint32_t)a.groups * 4u;
+    x_at = (uint32_t)(across * MT * 4 + j) * (uint32_t)a.x_stride * 2u + c * 16;
+    x_four = (uint32_t)a.x_stride * 8u;
+    clear();
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) y[t][mt] = f32x4{0, 0, 0, 0};
+  }
+  struct Groups {
+    int g, left;
+  };
+  __device__ __forceinline__ Groups groups_at(int kb) const {
+    const int g = kb / a.group;
+    return Groups{g, (g + 1) * a.group - kb};
+  }
+  __device__ __forceinline__ void load(Step& st, int kb, bool there, Groups& at) const {
+    const uint32_t wk = there ? w_at + (uint32_t)kb / 2u : kNowhere;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) st.w[t] = w_buf.load16(wk + t * w_tile);
+#pragma unroll
+    for (int i = 0; i < PARTS; ++i) {
+      const uint32_t g = min(at.g, a.groups - 1);
+      st.s[i] = WIDE ? s_buf.load4(there ? s_at + g * 4u : kNowhere) : s_buf.load2(there ? s_at + g * 2u : kNowhere);
+      st.z[i] = z_buf.load4(there ? z_at + g * 4u : kNowhere);
+      at.left -= SMALL ? 32 : kStepK;
+      const int over = (int)((uint32_t)(at.left - 1) >> 31);
+      at.left += -over & a.group, at.g += over;
+    }
+  }
+  __device__ __forceinline__ void load_rows(Vec<uint32_t, 4>* x, int kb, bool there) const {
+    const uint32_t xk = (int)there & (int)(kb + c * 8 < a.k) ? x_at + (uint32_t)kb * 2u : kNowhere;
+#pragma unroll
+    for (int i = 0; i < MT; ++i) x[i] = x_buf.load16(xk + i * x_four);
+  }
+  __device__ __forceinline__ void store_rows(const Vec<uint32_t, 4>* x, Vec<uint32_t, 4>* lds) const {
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const int r = across * MT * 4 + i * 4 + j;
+      lds[r * 16 + (c ^ (r & 15))] = x[i];
+    }
+  }
+
+  // x(mt, t): the operand of rows 16 mt ..., columns 32 t ... of the step
+  template <bool SIGNED, typename X>
+  __device__ __forceinline__ void step(Step& st, X x) {
+    const Operand ones = T::id == CTMI_BF16 ? Operand{{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u}}
+                                            : Operand{{0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u}};
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) transpose4(st.w[nt].v);
+    f32x4 acc[NT][MT], sums[MT];
+    float s[NT], z[NT];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      if (SMALL || t == 0) {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) sums[mt] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const uint32_t raw = __shfl(st.s[t], nt * 16 + c, kWave), zeros = __shfl(st.z[t], nt * 2 + (c >> 3), kWave);
+          s[nt] = WIDE ? u2f(raw) : T::to_f32((uint16_t)raw);
+          z[nt] = (float)(((zeros >> (4 * (c & 7))) & 15u) | z_none);
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) acc[nt][mt] = f32x4{0, 0, 0, 0};
+        }
+      }
+      Operand w[NT];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) w[nt] = SIGNED ? signed_codes_of<T>(st.w[nt].v[t], z[nt]) : codes_of<T>(st.w[nt].v[t]);
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        const Operand v = x(mt, t);
+        if constexpr (!SIGNED) sums[mt] = product<T>(v, ones, sums[mt]);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) acc[nt][mt] = product<T>(v, w[nt], acc[nt][mt]);
+      }
+      if (SMALL || t == 3) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              y[nt][mt][i] = fmaf(s[nt], SIGNED ? acc[nt][mt][i] : fmaf(-z[nt], sums[mt][i], acc[nt][mt][i]), y[nt][mt][i]);
+      }
+    }
+  }
+
+  // columns k0 ... k0 + wave_k - 1, as far as there are any; the 4 wavefronts that share x, and
+  // with them the workgroup, go through the same steps
+  __device__ __forceinline__ void run(int k0, int k1, Vec<uint32_t, 4>* lds) {
+    constexpr int TILE = MT * 16 * 16;
+    Step one, two;
+    Vec<uint32_t, 4> rows[MT];
+    Groups at = groups_at(min(k0, a.k - 1));
+    load_rows(rows, k0, k0 < k1);
+    load(one, k0, k0 < k1, at);
+    store_rows(rows, lds);
+    load_rows(rows, k0 + kStepK, k0 + kStepK < k1);
+    load(two, k0 + kStepK, k0 + kStepK < k1, at);
+    __syncthreads();
+    auto from = [&](const Vec<uint32_t, 4>* tile) {
+      return [tile, this](int mt, int t) { return __builtin_bit_cast(Operand, tile[(mt * 16 + c) * 16 + ((t * 4 + j) ^ c)]); };
+    };
+#pragma unroll 1
+    for (int kb = k0; kb < k0 + a.wave_k; kb += 2 * kStepK) {
+      step<false>(one, from(lds));
+      store_rows(rows, lds + TILE);
+      load_rows(rows, kb + 2 * kStepK, kb + 2 * kStepK < k1);
+      load(one, kb + 2 * kStepK, kb + 2 * kStepK < k1, at);
+      __syncthreads();
+      step<false>(two, from(lds + TILE));
+      store_rows(rows, lds);
+      load_rows(rows, kb + 3 * kStepK, kb + 3 * kStepK < k1);
+      load(two, kb + 3 * kStepK, kb + 3 * kStepK < k1, at);
+      __syncthreads();
+    }
+  }
+
+  // the same by one wavefront alone, x from where it lies
+  __device__ __forceinline__ void run_signed(int k0, int k1) {
+    clear();
+#pragma unroll 1
+    for (int kb = k0; kb < k1; kb += kStepK) {
+      Step st;
+      Groups at = groups_at(kb);
+      load(st, kb, true, at);
+      step<true>(st, [&](int mt, int t) {
+        const int k = kb + t * 32 + j * 8;
+        return __builtin_bit_cast(Operand, x_buf.load16(k < a.k ? (uint32_t)(mt * 16 + c) * (uint32_t)a.x_stride * 2u + k * 2u : kNowhere));
+      });
+    }
+  }
+};
+
+template <typename T, int MT, int NT, bool SMALL, bool WIDE>
+__global__ __launch_bounds__(8 * kWave, 2) void packed_linear_shared_kernel(LinearArgs a) {
+  using Wave = LinearShared<T, MT, NT, SMALL, WIDE>;
+  constexpr int TM = MT * 16, TN = Wave::ACROSS * NT * 16;
+  extern __shared__ Vec<uint32_t, 4> lds[];  // x: two steps for each half of k; then sums [TM][TN]
+  const int wave = threadIdx.x / kWave, across = wave % Wave::ACROSS, along = wave / Wave::ACROSS;
+  const int n0 = blockIdx.x * TN, m0 = blockIdx.y * TM;
+  Wave w(a, n0 + across * NT * 16, m0, across);
+  const int64_t begin = ((int64_t)blockIdx.z * Wave::ALONG + along) * a.wave_k;
+  const int k0 = (int)(begin < a.k ? begin : a.k), k1 = (int)(begin + a.wave_k < a.k ? begin + a.wave_k : a.k);
+  w.run(k0, k1, lds + along * 2 * MT * 16 * 16);
+  bool bad = false;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) bad |= !(fabsf(w.y[nt][mt][i]) <= 3.4028235e38f);
+  if (__any(bad)) w.run_signed(k0, k1);
+  float* meet = (float*)lds;
+  const int rows = min(TM, a.m - m0);
+#pragma unroll
+  for (int half = 1; half >= 0; --half) {
+    if (along == half) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float* at = &meet[(mt * 16 + w.j * 4 + i) * TN + across * NT * 16 + nt * 16 + w.c];
+            *at = half == 1 ? w.y[nt][mt][i] : *at + w.y[nt][mt][i];
+          }
+    }
+    __syncthreads();
+  }
+  for (int at = threadIdx.x; at < rows * TN; at += 8 * kWave) {
+    const int r = at / TN, n = n0 + at % TN;
+    if (n < a.n) {
+      const int64_t cell = (int64_t)(m0 + r) * a.n + n;
+      if (a.part) a.part[(int64_t)blockIdx.z * a.m * a.n + cell] = meet[at];
+      else a.out[cell] = T::from_f32(meet[at] + (a.bias ? T::to_f32(a.bias[n]) : 0.0f));
+    }
+  }
+}
+
 template <typename T>
 __global__ __launch_bounds__(256) void packed_linear_join_kernel(LinearArgs a, int splits) {
   const int64_t cells = (int64_t)a.m * a.n;
@@ -392,21 +610,30 @@ struct LinearLaunch {
   int64_t splits, wave_k;
 };
 
+// More than 16 rows go to the shared kernel where rows of weight and x are whole 16-byte pieces;
+// otherwise they are taken 16 at a time.
 LinearLaunch plan_linear(int64_t m, int64_t n, int64_t k) {
   LinearLaunch l;
-  l.mt = m <= 16 ? 1 : m <= 32 ? 2 : 4;
-  const int64_t tiles = cdiv(n, 16), m_blocks = cdiv(m, l.mt * 16);
+  const int64_t tiles = cdiv(n, 16);
   l.splits = 1;
-  if (l.mt == 1) {
+  if (m <= 16 || k % 32 != 0) {
+    l.mt = 1;
     l.nt = tiles >= 1024 ? 4 : tiles >= 512 ? 2 : 1;
     l.waves = l.nt == 4 ? 4 : 8;
+    l.wave_k = cdiv(cdiv(k, l.waves), kStepK) * kStepK;
   } else {
-    l.nt = l.mt == 4 ? 2 : 4;
-    l.waves = 4;
-    const int64_t units = cdiv(tiles, l.nt) * m_blocks;
-    while (units * l.splits < 512 && k / (l.waves * l.splits * 2) >= 256 && l.splits < 16) l.splits *= 2;
+    l.mt = m <= 32 ? 2 : 4;
+    l.nt = 2;
+    l.waves = 8;
+    // one workgroup per compute unit; a split's sums leave and come back in fp32, so no more
+    // of them than it takes, of 256 columns at least
+    const int64_t units = cdiv(tiles, 8) * cdiv(m, l.mt * 16);
+    if (units < 256) l.splits = 256 / units;
+    if (l.splits > k / 512) l.splits = k / 512 > 0 ? k / 512 : 1;
+    if (l.splits > 16) l.splits = 16;
+    l.wave_k = cdiv(cdiv(k, 2 * l.splits), 2 * kStepK) * 2 * kStepK;
+    l.splits = cdiv(k, 2 * l.wave_k);
   }
-  l.wave_k = cdiv(cdiv(k, l.waves * l.splits), kStepK) * kStepK;
   return l;
 }
 
@@ -447,43 +674,50 @@ extern "C" int ctmi_packed_linear(const void* x, int32_t x_dtype, int64_t x_stri
   const int64_t need = l.splits > 1 ? l.splits * m * n * 4 : 0;
   CTMI_REQUIRE(tmp_bytes >= need && (need == 0 || (tmp != nullptr && (uintptr_t)tmp % 16 == 0)), CTMI_ERR_VALUE,
                "tmp needs %lld bytes at a 16-byte boundary, has %lld", (long long)need, (long long)tmp_bytes);
-  const int64_t tm = l.mt * 16, tn = l.nt * 16;
+  const int64_t tm = l.mt * 16, tn = l.nt * 16 * (l.mt == 1 ? 1 : 4);
   CTMI_REQUIRE(cdiv(m, tm) < (1 << 16), CTMI_ERR_UNSUPPORTED, "too many rows: %lld", (long long)m);
+  const bool aligned = k % 32 == 0 && (uintptr_t)packed % 16 == 0;
+  CTMI_REQUIRE(aligned || l.mt == 1, CTMI_ERR_VALUE, "weight_packed must be 16-byte aligned for more than 16 rows");
   LinearArgs a{(const uint16_t*)x, x_stride, (const uint32_t*)packed, scale, (const uint32_t*)zero_point,
                (const uint16_t*)bias, (uint16_t*)out, need ? (float*)tmp : nullptr, (int32_t)m, (int32_t)n,
-               (int32_t)k, (int32_t)group, (int32_t)(k / group), (int32_t)cdiv(k, 8), (int32_t)l.wave_k};
+               (int32_t)k, (int32_t)group, (int32_t)(k / group), (int32_t)cdiv(k, 8), (int32_t)l.wave_k, aligned};
   const dim3 grid((unsigned)cdiv(n, tn), (unsigned)cdiv(m, tm), (unsigned)l.splits), threads(l.waves * kWave);
-  const size_t lds = (size_t)l.waves * tm * (tn * 4 > 256 ? tn * 4 : 256);
+  const size_t lds = l.mt == 1 ? (size_t)l.waves * 16 * (tn * 4 > 256 ? tn * 4 : 256) : (size_t)l.mt * 16 * 256 * 4;
   const hipStream_t s = (hipStream_t)stream;
   const bool small = group % kStepK != 0 && group != k;
-#define LAUNCH(T, MT, NT, XL, W, P)                                                                   \
-  do {                                                                                                \
-    if (scale_dtype == CTMI_F32) {                                                                    \
-      if (small) packed_linear_kernel<T, MT, NT, XL, true, true, W, P><<<grid, threads, lds, s>>>(a);  \
-      else packed_linear_kernel<T, MT, NT, XL, false, true, W, P><<<grid, threads, lds, s>>>(a);       \
-    } else {                                                                                          \
-      if (small) packed_linear_kernel<T, MT, NT, XL, true, false, W, P><<<grid, threads, lds, s>>>(a); \
-      else packed_linear_kernel<T, MT, NT, XL, false, false, W, P><<<grid, threads, lds, s>>>(a);      \
-    }                                                                                                 \
+#define BY_SCALE(KERNEL, ...)                                                       \
+  do {                                                                              \
+    if (scale_dtype == CTMI_F32) KERNEL(__VA_ARGS__, true);                         \
+    else KERNEL(__VA_ARGS__, false);                                                \
   } while (0)
+#define BY_GROUP(KERNEL, ...)                                                       \
+  do {                                                                              \
+    if (small) BY_SCALE(KERNEL, __VA_ARGS__, true);                                 \
+    else BY_SCALE(KERNEL, __VA_ARGS__, false);                                      \
+  } while (0)
+#define FEW(T, NT, XL, W, P, SMALL, WIDE) packed_linear_kernel<T, 1, NT, XL, SMALL, WIDE, W, P><<<grid, threads, lds, s>>>(a)
+#define MANY(T, MT, SMALL, WIDE) packed_linear_shared_kernel<T, MT, 2, SMALL, WIDE><<<grid, threads, lds, s>>>(a)
 #define BY_SIZE(T)                                  \
   do {                                              \
-    if (l.mt == 4) LAUNCH(T, 4, 2, 16, 4, 2);       \
-    else if (l.mt == 2) LAUNCH(T, 2, 4, 8, 4, 2);   \
+    if (l.mt == 4) BY_GROUP(MANY, T, 4);            \
+    else if (l.mt == 2) BY_GROUP(MANY, T, 2);       \
     else if (m > 4) {                               \
-      if (l.nt == 4) LAUNCH(T, 1, 4, 4, 4, 3);      \
-      else if (l.nt == 2) LAUNCH(T, 1, 2, 4, 8, 4); \
-      else LAUNCH(T, 1, 1, 4, 8, 4);                \
+      if (l.nt == 4) BY_GROUP(FEW, T, 4, 4, 4, 3);  \
+      else if (l.nt == 2) BY_GROUP(FEW, T, 2, 4, 8, 4); \
+      else BY_GROUP(FEW, T, 1, 4, 8, 4);            \
     } else {                                        \
-      if (l.nt == 4) LAUNCH(T, 1, 4, 1, 4, 4);      \
-      else if (l.nt == 2) LAUNCH(T, 1, 2, 1, 8, 4); \
-      else LAUNCH(T, 1, 1, 1, 8, 4);                \
+      if (l.nt == 4) BY_GROUP(FEW, T, 4, 1, 4, 3);  \
+      else if (l.nt == 2) BY_GROUP(FEW, T, 2, 1, 8, 4); \
+      else BY_GROUP(FEW, T, 1, 1, 8, 4);            \
     }                                               \
     if (need) packed_linear_join_kernel<T><<<dim3((unsigned)(cdiv(m * n, 256) < 2048 ? cdiv(m * n, 256) : 2048)), dim3(256), 0, s>>>(a, (int)l.splits); \
   } while (0)
   if (x_dtype == CTMI_BF16) BY_SIZE(BF16);
   else BY_SIZE(F16);
 #undef BY_SIZE
-#undef LAUNCH
+#undef MANY
+#undef FEW
+#undef BY_GROUP
+#undef BY_SCALE
   return check_launch("packed_linear");
 }
