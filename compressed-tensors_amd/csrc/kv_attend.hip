@@ -241,6 +241,12 @@ struct AttendRows {
           for (int i = 0; i < 4; ++i) s[t][kt][i] = !valid || at16 + kt * 4 + i >= ends[t] ? -INFINITY : s[t][kt][i] * ks;
     }
     Operand hi[RT][2], lo[RT][2];
+    auto weights = [](uint32_t& high, uint32_t& low, float w0, float w1) {
+      high = pack_bf16x2(w0, w1);
+      if constexpr (SPLIT) low = pack_bf16x2(w0 - u2f(high << 16), w1 - u2f(high & 0xFFFF0000u));
+    };
+    const bool plain = __all(vs > 0x1p-30f && vs < 0x1p30f);
+    const float log_vs = __builtin_amdgcn_logf(vs), by_vs = __builtin_amdgcn_rcpf(vs);
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
       float m = s[t][0][0];
@@ -260,20 +266,33 @@ struct AttendRows {
         for (int d = 0; d < DT; ++d) o[t][d] *= shrink;
       }
       const float base = top[t] == -INFINITY ? 0.0f : top[t];
-      // the scale of a block that a row sees nothing of does not touch it, whatever it is
-      const float by = whole || (valid && at16 < ends[t]) ? vs : 0.0f;
+      if (plain) {
+        // weight times scale in one exponential; the sum of weights takes the scale out again
+        const float less = base - log_vs;
+        float part = 0.0f;
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float p0 = exp2_fast(fmaf(s[t][u * 2 + e / 2][(e % 2) * 2], unit, -base));
-          const float p1 = exp2_fast(fmaf(s[t][u * 2 + e / 2][(e % 2) * 2 + 1], unit, -base));
-          sum[t] += p0 + p1;
-          const float w0 = p0 * by, w1 = p1 * by;
-          hi[t][u].w[e] = pack_bf16x2(w0, w1);
-          if constexpr (SPLIT)
-            lo[t][u].w[e] = pack_bf16x2(w0 - u2f(hi[t][u].w[e] << 16), w1 - u2f(hi[t][u].w[e] & 0xFFFF0000u));
-        }
+          for (int e = 0; e < 4; ++e) {
+            const float w0 = exp2_fast(fmaf(s[t][u * 2 + e / 2][(e % 2) * 2], unit, -less));
+            const float w1 = exp2_fast(fmaf(s[t][u * 2 + e / 2][(e % 2) * 2 + 1], unit, -less));
+            part += w0 + w1;
+            weights(hi[t][u].w[e], lo[t][u].w[e], w0, w1);
+          }
+        sum[t] = fmaf(part, by_vs, sum[t]);
+      } else {
+        // the scale of a block that a row sees nothing of does not touch it, whatever it is
+        const float by = whole || (valid && at16 < ends[t]) ? vs : 0.0f;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float p0 = exp2_fast(fmaf(s[t][u * 2 + e / 2][(e % 2) * 2], unit, -base));
+            const float p1 = exp2_fast(fmaf(s[t][u * 2 + e / 2][(e % 2) * 2 + 1], unit, -base));
+            sum[t] += p0 + p1;
+            weights(hi[t][u].w[e], lo[t][u].w[e], p0 * by, p1 * by);
+          }
+      }
     }
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
@@ -334,8 +353,8 @@ struct AttendUnit {
     id /= a.kv_heads;
     chunk = id % a.chunks;
     id /= a.chunks;
-    tile = a.tiles - 1 - id % a.tiles;  // the rows that see most come first
-    r = id / a.tiles;
+    r = id % a.requests;
+    tile = a.tiles - 1 - id / a.requests;  // the rows that see most come first
   }
 };
 
@@ -479,7 +498,10 @@ __global__ __launch_bounds__(kAttendWaves* kWave, D == 256 || RT == 2 ? 1 : 2) v
 // (measured at 2 x 2000 queries over 4000 keys: 455 us).  Pieces of a row are swapped in LDS
 // by some bits of the row's number, so that the rows that are read together lie in different
 // banks.
-template <typename T, bool FP8, int D, int RT, bool SPLIT>
+//
+// WIDE: blocks are whole steps of 64 keys, so a step lies in one of them: its number, its
+// addresses and scales are the wavefront's and cost no vector instruction.
+template <typename T, bool FP8, int D, int RT, bool SPLIT, bool WIDE>
 __global__ __launch_bounds__(kAttendWaves* kWave, D == 256 ? 1 : 2) void kv_attend_rows_kernel(AttendArgs a) {
   using Rows = AttendRows<T, FP8, D, RT, SPLIT>;
   constexpr int ROWS = kAttendWaves * RT * 16, PIECES = D / 64;  // 16-byte pieces a thread loads of either
@@ -512,24 +534,43 @@ __global__ __launch_bounds__(kAttendWaves* kWave, D == 256 ? 1 : 2) void kv_atte
     int bk[PIECES], ak[PIECES], bv, av, bs_next = 0;  // blocks of the step to load; bs: of this lane's 16 keys
     const int my_key = threadIdx.x / KP, my_piece = threadIdx.x % KP, my_group = threadIdx.x % 4, my_d = threadIdx.x / 4;
     auto find = [&](int kb) {
+      if constexpr (WIDE) {
+        bv = __builtin_amdgcn_readfirstlane(look_up(a, r, __builtin_amdgcn_readfirstlane(kb), &av));
+        av = __builtin_amdgcn_readfirstlane(av);
+      } else {
 #pragma unroll
-      for (int p = 0; p < PIECES; ++p) {
-        const int key = kb + my_key + p * KEYS;
-        bk[p] = look_up(a, r, key, &ak[p]);
-        ak[p] += key & 15;
+        for (int p = 0; p < PIECES; ++p) {
+          const int key = kb + my_key + p * KEYS;
+          bk[p] = look_up(a, r, key, &ak[p]);
+          ak[p] += key & 15;
+        }
+        bv = look_up(a, r, kb + my_group * 16, &av);
       }
-      bv = look_up(a, r, kb + my_group * 16, &av);
     };
+    const uint32_t key_at = threadIdx.x * 16, value_at = my_d * a.block_size + my_group * 16, value_step = 64 * a.block_size;
     auto load = [&] {
+      if constexpr (WIDE) {
+        const int64_t cell = cell_of(a, bv, kv);
+        const uint8_t *k = a.key + cell * bytes + av * D, *v = a.value + cell * bytes + av;
 #pragma unroll
-      for (int p = 0; p < PIECES; ++p)
-        kr[p] = ldg<uint32_t, 4>((const uint32_t*)(a.key + cell_of(a, bk[p], kv) * bytes + ak[p] * D + my_piece * 16));
-      const uint8_t* v = a.value + cell_of(a, bv, kv) * bytes + my_d * a.block_size + av;
+        for (int p = 0; p < PIECES; ++p) {
+          kr[p] = ldg<uint32_t, 4>((const uint32_t*)(k + (key_at + p * kAttendWaves * kWave * 16)));
+          vr[p] = ldg<uint32_t, 4>((const uint32_t*)(v + (value_at + p * value_step)));
+        }
+        bs_next = bv;
+        ks = a.key_scale[cell] * a.scale;
+        vs = a.value_scale[cell];
+      } else {
 #pragma unroll
-      for (int p = 0; p < PIECES; ++p) vr[p] = ldg<uint32_t, 4>((const uint32_t*)(v + p * 64 * a.block_size));
-      bs_next = __shfl(bv, j, kWave);  // lane j's group is j
-      ks = a.key_scale[cell_of(a, bs_next, kv)] * a.scale;
-      vs = a.value_scale[cell_of(a, bs_next, kv)];
+        for (int p = 0; p < PIECES; ++p)
+          kr[p] = ldg<uint32_t, 4>((const uint32_t*)(a.key + cell_of(a, bk[p], kv) * bytes + ak[p] * D + my_piece * 16));
+        const uint8_t* v = a.value + cell_of(a, bv, kv) * bytes + value_at - my_group * 16 + av;
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p) vr[p] = ldg<uint32_t, 4>((const uint32_t*)(v + p * value_step));
+        bs_next = __shfl(bv, j, kWave);  // lane j's group is j
+        ks = a.key_scale[cell_of(a, bs_next, kv)] * a.scale;
+        vs = a.value_scale[cell_of(a, bs_next, kv)];
+      }
     };
     auto store = [&](int half) {
 #pragma unroll
@@ -742,7 +783,10 @@ extern "C" int ctmi_kv_attend(const void* q, int32_t dtype, int64_t q_token_stri
 #define BY_TILE(T, F, D)                                                                                           \
   do {                                                                                                             \
     constexpr int RT2 = D == 256 ? 1 : 2;                                                                          \
-    if (!l.split_keys) kv_attend_rows_kernel<T, F, D, RT2, T::id == CTMI_F16><<<blocks_of, threads, 0, s>>>(a);    \
+    if (!l.split_keys && a.block_size % kStep == 0)                                                                \
+      kv_attend_rows_kernel<T, F, D, RT2, T::id == CTMI_F16, true><<<blocks_of, threads, 0, s>>>(a);               \
+    else if (!l.split_keys)                                                                                        \
+      kv_attend_rows_kernel<T, F, D, RT2, T::id == CTMI_F16, false><<<blocks_of, threads, 0, s>>>(a);              \
     else if (RT2 == 1 || l.row_tiles == 1) kv_attend_split_kernel<T, F, D, 1><<<blocks_of, threads, 0, s>>>(a);    \
     else kv_attend_split_kernel<T, F, D, RT2><<<blocks_of, threads, 0, s>>>(a);                                    \
     if (cells) kv_attend_join_kernel<T, D><<<dim3((unsigned)join), threads, 0, s>>>(a, l.tile_rows, (int)max_query); \
