@@ -294,10 +294,16 @@ struct AttendRows {
           }
       }
     }
+    // (two loops: a branch for each d would leave each load of a value alone with its wait)
+    if (whole) gather(hi, lo, value);
+    else gather(hi, lo, [&](int d) { return clean(value(d), true); });
+  }
+
+  template <typename Value>
+  __device__ __forceinline__ void gather(const Operand (*hi)[2], const Operand (*lo)[2], Value value) {
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
-      Vec<uint32_t, 4> w = value(d);
-      if (!whole) w = clean(w, true);
+      const Vec<uint32_t, 4> w = value(d);
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const Operand v = widen8<BF16, FP8>(w.v[2 * u], w.v[2 * u + 1]);
