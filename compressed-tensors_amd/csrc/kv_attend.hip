@@ -145,8 +145,9 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
 }
 
 // The rows of a wavefront and what they have gathered: RT tiles of 16, row `first` + 16 t + c
-// in lanes with lane % 16 == c.
-template <typename T, bool FP8, int D, int RT, bool SPLIT>
+// in lanes with lane % 16 == c.  UNIFORM: a step lies in one block, so its scales are one
+// number, and `sum` is the row's in all its lanes; otherwise each lane group has a part of it.
+template <typename T, bool FP8, int D, int RT, bool SPLIT, bool UNIFORM>
 struct AttendRows {
   static constexpr int CH = D / 64;  // 16-byte pieces of a key per lane
   static constexpr int DT = D / 16;  // tiles of the output's dimensions
@@ -254,11 +255,12 @@ struct AttendRows {
       for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
         for (int i = 0; i < 4; ++i) m = fmaxf(m, s[t][kt][i]);
-      m = groups_max(m * unit);
+      m *= unit;
       // weights may exceed 1 by 2^8 before the sums are brought to a new maximum: fp32 and
-      // bf16 keep their relative precision there
+      // bf16 keep their relative precision there, and the lanes of a row need not be asked
+      // for their maximum in most steps
       if (__any(m > top[t] + 8.0f)) {
-        const float now = fmaxf(top[t], m);
+        const float now = fmaxf(top[t], groups_max(m));
         const float shrink = top[t] == -INFINITY ? 0.0f : exp2_fast(top[t] - now);
         top[t] = now;
         sum[t] *= shrink;
@@ -276,22 +278,35 @@ struct AttendRows {
           for (int e = 0; e < 4; ++e) {
             const float w0 = exp2_fast(fmaf(s[t][u * 2 + e / 2][(e % 2) * 2], unit, -less));
             const float w1 = exp2_fast(fmaf(s[t][u * 2 + e / 2][(e % 2) * 2 + 1], unit, -less));
-            part += w0 + w1;
+            if constexpr (!UNIFORM) part += w0 + w1;
             weights(hi[t][u].w[e], lo[t][u].w[e], w0, w1);
           }
+        if constexpr (UNIFORM) {
+          // all weights carry the same scale: their sum is two products with ones
+          const Operand ones = {{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u}};
+          f32x4 all = {0, 0, 0, 0};
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            all = product<BF16>(ones, hi[t][u], all);
+            if constexpr (SPLIT) all = product<BF16>(ones, lo[t][u], all);
+          }
+          part = all[0];
+        }
         sum[t] = fmaf(part, by_vs, sum[t]);
       } else {
         // the scale of a block that a row sees nothing of does not touch it, whatever it is
         const float by = whole || (valid && at16 < ends[t]) ? vs : 0.0f;
+        float part = 0.0f;
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float p0 = exp2_fast(fmaf(s[t][u * 2 + e / 2][(e % 2) * 2], unit, -base));
             const float p1 = exp2_fast(fmaf(s[t][u * 2 + e / 2][(e % 2) * 2 + 1], unit, -base));
-            sum[t] += p0 + p1;
+            part += p0 + p1;
             weights(hi[t][u].w[e], lo[t][u].w[e], p0 * by, p1 * by);
           }
+        sum[t] += UNIFORM ? groups_sum(part) : part;
       }
     }
     // (two loops: a branch for each d would leave each load of a value alone with its wait)
@@ -346,7 +361,8 @@ struct AttendRows {
 
   __device__ __forceinline__ void finish() {
 #pragma unroll
-    for (int t = 0; t < RT; ++t) sum[t] = groups_sum(sum[t]);
+    for (int t = 0; t < RT; ++t)
+      if constexpr (!UNIFORM) sum[t] = groups_sum(sum[t]);
   }
 };
 
@@ -380,7 +396,7 @@ __device__ __forceinline__ int64_t cell_of(const AttendArgs& a, int block, int k
 // from memory into the registers they are multiplied from
 template <typename T, bool FP8, int D, int RT>
 __global__ __launch_bounds__(kAttendWaves* kWave, D == 256 || RT == 2 ? 1 : 2) void kv_attend_split_kernel(AttendArgs a) {
-  using Rows = AttendRows<T, FP8, D, RT, true>;
+  using Rows = AttendRows<T, FP8, D, RT, true, false>;
   constexpr int ROWS = RT * 16, CH = Rows::CH, DT = Rows::DT;
   const int lane = lane_id(), wave = threadIdx.x / kWave, c = lane & 15, j = lane >> 4;
   const int share = a.q_heads / a.kv_heads;
@@ -509,7 +525,7 @@ __global__ __launch_bounds__(kAttendWaves* kWave, D == 256 || RT == 2 ? 1 : 2) v
 // addresses and scales are the wavefront's and cost no vector instruction.
 template <typename T, bool FP8, int D, int RT, bool SPLIT, bool WIDE>
 __global__ __launch_bounds__(kAttendWaves* kWave, D == 256 ? 1 : 2) void kv_attend_rows_kernel(AttendArgs a) {
-  using Rows = AttendRows<T, FP8, D, RT, SPLIT>;
+  using Rows = AttendRows<T, FP8, D, RT, SPLIT, WIDE>;
   constexpr int ROWS = kAttendWaves * RT * 16, PIECES = D / 64;  // 16-byte pieces a thread loads of either
   constexpr int KP = D / 16;                                     // pieces of a key
   constexpr int KEYS = kAttendWaves * kWave / KP;                // keys per round of loads

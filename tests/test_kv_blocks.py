@@ -7,8 +7,10 @@ its weight p = exp(score - top) by that (twice: its own and the top's share in t
 2^-20 for the exponential and the argument's rounding; weights enter the second product as a
 sum of two bf16 numbers (off by 2^-16 of themselves) or, for bf16 outputs, one (eps / 2 =
 2^-8: bf16 has 8 significant bits, its neighbours in [1, 2) are 2^-7 apart); sums
-over n keys pass n / 32 + 96 additions.  All of it scales with sum p |v|, and the output's
-rounding is eps / 2 of the value.
+over n keys pass n / 32 + 96 additions.  All of it scales with sum p |v|.  Where the weights
+are divided by the sum of the rounded weights, w' = w (1 + d) with |d| <= e, the quotient is
+sum p (1 + d) v / sum p (1 + d): off by at most e sum p |v| above and, through the sum below,
+by e / (1 - e) |o| once more.  The output's rounding is eps / 2 of the value.
 """
 import pytest
 import torch
@@ -45,7 +47,7 @@ def check_attention(got, q, blocks, table, lens, starts, scale=None, out=None):
     eps, n = torch.finfo(got.dtype).eps, max(int(max(lens)) if len(lens) else 0, 1)
     weight = 2.0 ** -8 if got.dtype is torch.bfloat16 else 2.0 ** -16
     rel = weight + 2.0 ** -20 + 2 * (q.shape[2] / 32 + 40) * 2.0 ** -24 * reach + (n / 32 + 96) * 2.0 ** -24
-    bound = eps / 2 * want.abs() + rel * mag + torch.finfo(got.dtype).smallest_normal * eps
+    bound = (eps / 2 + 1.004 * weight) * want.abs() + rel * mag + torch.finfo(got.dtype).smallest_normal * eps
     off = (got.cpu().double() - want).abs()
     assert (off <= bound).all(), f"{(off / bound).max().item():.3g} times the bound"
 
