@@ -213,7 +213,10 @@ struct AttendRows {
       }
     }
 
+    // the wavefront that multiplies goes before the one that weighs: the matrix cores wait for
+    // neither (2 x 2000 of 4000: 266 us without, 253 with)
     f32x4 s[RT][4];
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int kt = 0; kt < 4; ++kt) {
 #pragma unroll
@@ -229,6 +232,7 @@ struct AttendRows {
         }
       }
     }
+    __builtin_amdgcn_s_setprio(0);
     keys_done();
 
     float unit = ks;  // what a score is still to be multiplied by
@@ -310,8 +314,10 @@ struct AttendRows {
       }
     }
     // (two loops: a branch for each d would leave each load of a value alone with its wait)
+    __builtin_amdgcn_s_setprio(1);
     if (whole) gather(hi, lo, value);
     else gather(hi, lo, [&](int d) { return clean(value(d), true); });
+    __builtin_amdgcn_s_setprio(0);
   }
 
   template <typename Value>
