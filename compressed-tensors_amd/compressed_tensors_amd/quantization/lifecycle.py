@@ -86,11 +86,12 @@ def disable_quantization(module: Module) -> None:
 
 
 def apply_quantization_config(model: Module, config: Optional[QuantizationConfig],
-                              run_compressed: bool = False):
+                              run_compressed: bool = False, keep_packed: bool = False):
     """attach the schemes of `config` to the modules they target and give these their
     scales and zero points (initialize_module_for_quantization); with run_compressed and a
     format other than dense a Linear becomes a CompressedLinear that holds the compressed
-    parameters.  A kv_cache_scheme goes onto every attention module."""
+    parameters, and with keep_packed one that multiplies with them as they are (4-bit
+    pack-quantized weights).  A kv_cache_scheme goes onto every attention module."""
     from compressed_tensors_amd.linear.compressed_linear import CompressedLinear
     from compressed_tensors_amd.modeling import initialize_hooked_attention, initialize_hooked_kv_cache
 
@@ -120,7 +121,8 @@ def apply_quantization_config(model: Module, config: Optional[QuantizationConfig
         module.quantization_scheme = scheme
         if (run_compressed and isinstance(module, torch.nn.Linear)
                 and config.format != CompressionFormat.dense.value):
-            CompressedLinear.from_linear(module, quantization_scheme=scheme, quantization_format=config.format)
+            CompressedLinear.from_linear(module, quantization_scheme=scheme, quantization_format=config.format,
+                                         keep_packed=keep_packed)
         else:
             if is_attention_module(module) and is_narrow_match(model, scheme.targets, name):
                 initialize_hooked_attention(model, module)

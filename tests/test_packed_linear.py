@@ -160,6 +160,70 @@ def test_captured_graph_and_streams(gpu):
     assert all(torch.equal(t, eager[1]) for t in on_side + here)
 
 
+def packed_module(dev, dtype, symmetric, strategy, bias=True, n=96, k=256, seed=0):
+    """a CompressedLinear that keeps its weight packed, filled with random codes"""
+    from compressed_tensors_amd import CompressedLinear
+    from compressed_tensors_amd.quantization import QuantizationArgs, QuantizationScheme
+
+    spec = dict(num_bits=4, type="int", symmetric=symmetric, strategy=strategy)
+    if strategy == "group":
+        spec["group_size"] = 64
+    layer = torch.nn.Linear(k, n, bias=bias).to(dtype).to(dev)
+    module = CompressedLinear.from_linear(layer, QuantizationScheme(targets=["Linear"], weights=QuantizationArgs(**spec)),
+                                          "pack-quantized", keep_packed=True)
+    _, packed, scale, zero, b = make(1, n, k, k // 64 if strategy == "group" else 1, dtype, asym=not symmetric, bias=bias, seed=seed)
+    module.weight_packed.data.copy_(packed)
+    module.weight_scale.data.copy_(scale)
+    module.weight_shape.data.copy_(torch.tensor([n, k]))
+    if zero is not None:
+        module.weight_zero_point.data.copy_(zero)
+    if bias:
+        module.bias.data.copy_(b)
+    return module, packed, scale, zero, b
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("symmetric,strategy,bias", [(True, "group", True), (False, "group", False), (False, "channel", True)])
+def test_compressed_linear_that_keeps_its_weight_packed(gpu, dtype, symmetric, strategy, bias):
+    from compressed_tensors_amd.config import QuantizationStatus
+
+    announce("keep_packed", dtype, symmetric, strategy, bias)
+    module, packed, scale, zero, b = packed_module(gpu, dtype, symmetric, strategy, bias)
+    for m in (1, 5, 40, 192):
+        x = torch.randn(m, 256).to(dtype)
+        with torch.no_grad():
+            check(module(x.to(gpu)), x, packed, scale, zero, b)
+    # many rows, and calls that are differentiated, go through the decompressed weight
+    dense = module.compressor.decompress_module(module)
+    x = torch.randn(193, 256).to(dtype).to(gpu)
+    with torch.no_grad():
+        assert torch.equal(module(x), torch.nn.functional.linear(x, dense, module.bias))
+    x = torch.randn(3, 256).to(dtype).to(gpu).requires_grad_()
+    y = module(x)
+    y.float().square().sum().backward()
+    other = x.detach().clone().requires_grad_()
+    torch.nn.functional.linear(other, dense, module.bias).float().square().sum().backward()
+    assert torch.equal(x.grad, other.grad)
+    assert module.quantization_status == QuantizationStatus.COMPRESSED and not hasattr(module, "weight")
+
+
+def test_keep_packed_refusals():
+    from compressed_tensors_amd import CompressedLinear
+    from compressed_tensors_amd.quantization import QuantizationArgs, QuantizationScheme
+
+    def convert(fmt="pack-quantized", k=256, **spec):
+        args = QuantizationArgs(**{**dict(num_bits=4, type="int", symmetric=True, strategy="group", group_size=64), **spec})
+        return CompressedLinear.from_linear(torch.nn.Linear(k, 32), QuantizationScheme(targets=["Linear"], weights=args), fmt,
+                                            keep_packed=True)
+
+    for bad in (dict(num_bits=8), dict(group_size=16), dict(group_size=64, k=96), dict(actorder="group"),
+                dict(fmt="int-quantized", num_bits=8, strategy="channel", group_size=None)):
+        with pytest.raises(NotImplementedError, match="keep_packed"):
+            convert(**bad)
+    assert convert().keep_packed and convert(actorder="weight").keep_packed
+
+
 def test_refusals():
     from compressed_tensors_amd.linear import packed_linear
 
