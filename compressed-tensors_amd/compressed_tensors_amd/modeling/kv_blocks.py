@@ -233,7 +233,9 @@ class BlockKVCache:
 
     A serving step is `plan(new_tokens, total)`, then for each layer `update(layer, key,
     value)` and `attend(layer, query)`.  Everything stays on the GPU: nothing here waits for
-    it except `check()`."""
+    it except `check()`.  A step that does not fit changes nothing: `update` then writes
+    nothing and `attend` leaves its rows as they are.  `plan` replaces the cache's tensors; a
+    captured graph calls the functions on buffers of its own."""
 
     def __init__(self, layers: int, num_blocks: int, max_requests: int, max_blocks_per_request: int,
                  kv_heads: int, head_dim: int, block_size: int = 64,
@@ -248,6 +250,17 @@ class BlockKVCache:
         self.num_free = torch.full((1,), num_blocks, dtype=torch.int32, device=device)
         self._step: Optional[KVPlan] = None
         self._longest: Optional[int] = None
+        self._calibrated = set()  # layers whose scales do not follow their values
+
+    def set_scales(self, layer: int, key_scale: Tensor, value_scale: Tensor) -> None:
+        """scales from calibration for all blocks of a layer: one, or one per kv head, as an
+        attention module holds them in `k_scale` / `v_scale` under a symmetric kv_cache_scheme of
+        8 bits.  `update` then keeps them and saturates.  For an empty cache."""
+        for scale, pool in zip((key_scale, value_scale), self.layers[layer][2:]):
+            if scale.numel() not in (1, pool.shape[1]):
+                raise ValueError(f"expected one scale or {pool.shape[1]}, got {tuple(scale.shape)}")
+            pool.copy_(scale.detach().reshape(1, -1).expand_as(pool))
+        self._calibrated.add(layer)
 
     def plan(self, new_tokens: Tensor, total_tokens: int, max_query: Optional[int] = None) -> KVPlan:
         """take the blocks for this step's tokens; `new_tokens` int32 [max_requests], -1 ends a
@@ -271,7 +284,7 @@ class BlockKVCache:
 
     def update(self, layer: int, key: Tensor, value: Tensor) -> None:
         """store this step's keys and values of one layer, [tokens, kv_heads, head_dim]"""
-        append_kv_blocks(key, value, self.layers[layer], self._current().slots)
+        append_kv_blocks(key, value, self.layers[layer], self._current().slots, dynamic=layer not in self._calibrated)
 
     def attend(self, layer: int, query: Tensor, softmax_scale: Optional[float] = None,
                max_seq: Optional[int] = None, out: Optional[Tensor] = None) -> Tensor:

@@ -411,6 +411,57 @@ def test_serving_steps_with_packed_projections(gpu, codes):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("codes,kind", [(FP8, "float"), (torch.int8, "int")])
+def test_cache_with_the_scales_of_a_calibrated_module(gpu, codes, kind):
+    """k_scale / v_scale of an attention module under a kv_cache_scheme: the codes are those
+    `quantize` gives with them"""
+    from compressed_tensors_amd.modeling import BlockKVCache
+    from compressed_tensors_amd.quantization import QuantizationArgs, quantize
+
+    cache = BlockKVCache(1, 4, 1, 4, 2, 64, 16, codes, device=gpu)
+    k_scale, v_scale = torch.tensor([0.011]).to(gpu), torch.tensor([0.02, 0.003]).view(2, 1, 1).to(gpu)
+    cache.set_scales(0, k_scale, v_scale)
+    with pytest.raises(ValueError):
+        cache.set_scales(0, torch.ones(3).to(gpu), v_scale)
+    k, v = torch.randn(20, 2, 64).bfloat16().to(gpu), torch.randn(20, 2, 64).bfloat16().to(gpu)
+    cache.plan(torch.tensor([20], dtype=torch.int32, device=gpu), 20)
+    cache.check()
+    cache.update(0, k, v)
+    args = QuantizationArgs(num_bits=8, type=kind, symmetric=True, strategy="tensor")
+    pool = cache.layers[0]
+    assert (pool.key_scale == 0.011).all() and (pool.value_scale[:, 1] == v_scale[1, 0, 0]).all()
+    for h in range(2):
+        for x, scale, got in ((k, k_scale, pool.key), (v, v_scale[h, 0], pool.value.transpose(2, 3))):
+            want = quantize(x[:, h].float(), scale, torch.zeros_like(scale), args, dtype=codes)
+            assert_bit_equal(got[:2, h].reshape(32, 64)[:20].contiguous().view(torch.uint8), want.cpu().view(torch.uint8), "codes")
+
+
+@pytest.mark.gpu
+def test_step_that_does_not_fit_changes_nothing(gpu):
+    from compressed_tensors_amd.modeling import BlockKVCache
+
+    cache = BlockKVCache(1, 2, 2, 4, 1, 64, 16, device=gpu)
+    with pytest.raises(ValueError, match="plan"):
+        cache.check()
+    cache.plan(torch.tensor([20, 0], dtype=torch.int32, device=gpu), 20)
+    cache.check()
+    before = [t.clone() for t in (cache.seq_lens, cache.block_table, cache.free_blocks, cache.num_free)]
+    cache.plan(torch.tensor([0, 17], dtype=torch.int32, device=gpu), 17)
+    with pytest.raises(RuntimeError, match="short of 2 blocks"):
+        cache.check()
+    codes = [t.view(torch.uint8).clone() for t in cache.layers[0]]
+    x = torch.randn(17, 1, 64).bfloat16().to(gpu)
+    cache.update(0, x, x)
+    out = torch.full_like(x, 3.0)
+    assert cache.attend(0, x, out=out) is out and (out == 3).all()
+    assert all(torch.equal(t.view(torch.uint8), c) for t, c in zip(cache.layers[0], codes))
+    assert all(torch.equal(a, b) for a, b in zip(before, (cache.seq_lens, cache.block_table, cache.free_blocks, cache.num_free)))
+    cache.plan(torch.tensor([0, 100], dtype=torch.int32, device=gpu), 100)
+    with pytest.raises(ValueError, match="longer than its row"):
+        cache.check()
+
+
+@pytest.mark.gpu
 def test_captured_decode_step(gpu):
     """a decode step in a graph, replayed over changed lengths, beside a second graph that shares
     the pool, with eager calls between the replays"""
