@@ -160,7 +160,7 @@ def append_kv_blocks(key: Tensor, value: Tensor, blocks: KVBlocks, slots: Tensor
 def _aligned(t: Tensor) -> Tensor:
     """`t` [tokens, heads, dim], or a copy if its heads do not start at 16-byte boundaries"""
     token, head, inner = t.stride()
-    if inner == 1 and head % 8 == 0 and token % 8 == 0 and t.data_ptr() % 16 == 0:
+    if inner == 1 and head % 8 == 0 and token % 8 == 0 and token < 1 << 22 and t.data_ptr() % 16 == 0:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 

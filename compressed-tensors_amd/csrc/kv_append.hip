@@ -99,10 +99,9 @@ __device__ __forceinline__ void append_window(const AppendArgs& a) {
   // rest of a longer run is read twice.
   constexpr int KEEP = 8;
   const int head = blockIdx.y, bs = a.block_size, lane = lane_id();
-  const int64_t stride = a.token_stride[side];
+  const int stride = (int)a.token_stride[side];
   const int64_t t0 = (int64_t)blockIdx.x * a.window;
-  __shared__ float peaks[2][kAppendThreads / kWave];
-  __shared__ int oddities[2][kAppendThreads / kWave];
+  __shared__ uint32_t peaks[2][kAppendThreads / kWave];
 
   // lane i holds the slot of token t0 - 1 + i: one look at them tells which tokens of the
   // window begin a run and, for all but the longest, how far it goes
@@ -138,28 +137,25 @@ __device__ __forceinline__ void append_window(const AppendArgs& a) {
       }
     }
 
-    const uint16_t* x = a.x[side] + t * stride + head * a.head_stride[side];
+    const uint16_t* x = a.x[side] + t * a.token_stride[side] + head * a.head_stride[side];
     // keys: piece i is 4 dimensions of token i / CH.  Values: item i is 4 dimensions of the 4
     // tokens of a word, of which those outside the run are read as its nearest; words of a row
     // of the block are lanes next to each other
     const int word0 = at / 4, words = (at + n + 3) / 4 - word0, items = side == 0 ? n * CH : words * CH;
     const uint32_t magic = 0xFFFFFFFFu / (uint32_t)words + 1;  // i / words for the i there are (words > 1)
     auto row_of = [&](int i) { return words == 1 ? i : (int)__umulhi((uint32_t)i, magic); };
-    auto key_piece = [&](int i) { return ldg<uint16_t, 4>(x + (i / CH) * stride + (i % CH) * 4); };
+    auto key_piece = [&](int i) { return ldg<uint16_t, 4>(x + (uint32_t)((i / CH) * stride + (i % CH) * 4)); };
     auto first_token = [&](int i) { return (word0 + i - row_of(i) * words) * 4 - at; };
     auto value_piece = [&](int i, int e) {
-      return ldg<uint16_t, 4>(x + min(max(first_token(i) + e, 0), n - 1) * stride + row_of(i) * 4);
+      return ldg<uint16_t, 4>(x + (uint32_t)(min(max(first_token(i) + e, 0), n - 1) * stride + row_of(i) * 4));
     };
-    float peak = 0.0f;
-    bool odd = false;
+    // magnitudes order like the unsigned integers of their bits, infinities and NaNs above all
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    u16x2 most = {0, 0};
     auto look = [&](const Vec<uint16_t, 4>& v) {
+      const Vec<uint32_t, 2> w = __builtin_bit_cast(Vec<uint32_t, 2>, v);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float m = fabsf(T::to_f32(v.v[e]));
-        const bool fine = m <= 3.4028235e38f;
-        peak = fmaxf(peak, fine ? m : 0.0f);
-        odd |= !fine;
-      }
+      for (int e = 0; e < 2; ++e) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, w.v[e] & 0x7FFF7FFFu));
     };
     Vec<uint16_t, 4> kept[KEEP];
 #pragma unroll
@@ -178,19 +174,32 @@ __device__ __forceinline__ void append_window(const AppendArgs& a) {
       for (int i = threadIdx.x + KEEP / 4 * kAppendThreads; i < items; i += kAppendThreads)
         for (int e = 0; e < 4; ++e) look(value_piece(i, e));
     }
-#pragma unroll
-    for (int m = 1; m < kWave; m *= 2) peak = fmaxf(peak, wave_shfl_xor(peak, m));
     // (the other half of peaks may still be read for the run before)
-    if (lane == 0) peaks[parity][threadIdx.x / kWave] = peak;
-    odd = __any(odd);
-    if (lane == 0) oddities[parity][threadIdx.x / kWave] = odd;
-    __syncthreads();
-    bool strange = false;
+    uint32_t high = most[0] > most[1] ? most[0] : most[1];
 #pragma unroll
-    for (int w = 0; w < kAppendThreads / kWave; ++w) {
-      peak = fmaxf(peak, peaks[parity][w]);
-      strange |= oddities[parity][w] != 0;
+    for (int m = 1; m < kWave; m *= 2) high = max(high, (uint32_t)wave_shfl_xor((int)high, m));
+    if (lane == 0) peaks[parity][threadIdx.x / kWave] = high;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kAppendThreads / kWave; ++w) high = max(high, peaks[parity][w]);
+    constexpr uint32_t kInfinity = T::id == CTMI_BF16 ? 0x7F80u : 0x7C00u;
+    const bool strange = high >= kInfinity;
+    if (strange) {  // the largest that is finite, element by element
+      high = 0;
+#pragma unroll 1
+      for (int i = threadIdx.x; i < n * D; i += kAppendThreads) {
+        const uint32_t m = x[(i / D) * stride + i % D] & 0x7FFFu;
+        high = m < kInfinity ? max(high, m) : high;
+      }
+#pragma unroll
+      for (int m = 1; m < kWave; m *= 2) high = max(high, (uint32_t)wave_shfl_xor((int)high, m));
+      __syncthreads();
+      if (lane == 0) peaks[parity][threadIdx.x / kWave] = high;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < kAppendThreads / kWave; ++w) high = max(high, peaks[parity][w]);
     }
+    const float peak = T::to_f32((uint16_t)high);
 
     float now = was;
     if (a.dynamic) {
@@ -289,6 +298,9 @@ extern "C" int ctmi_kv_append(const void* key, const void* value, int32_t dtype,
   CTMI_REQUIRE((key_token_stride | key_head_stride | value_token_stride | value_head_stride) % 8 == 0 &&
                    ((uintptr_t)key | (uintptr_t)value) % 16 == 0,
                CTMI_ERR_VALUE, "keys and values must be 16-byte aligned, token by token and head by head");
+  CTMI_REQUIRE(key_token_stride >= 0 && key_token_stride < (1 << 22) && value_token_stride >= 0 &&
+                   value_token_stride < (1 << 22),
+               CTMI_ERR_UNSUPPORTED, "tokens more than 2^22 elements apart");
   CTMI_REQUIRE(blocks->num_blocks * blocks->block_size < (1ll << 31), CTMI_ERR_UNSUPPORTED,
                "a pool must have fewer than 2^31 slots");
   const uint32_t sixteenths = blocks->block_size / 16;

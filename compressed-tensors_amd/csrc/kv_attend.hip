@@ -772,9 +772,9 @@ extern "C" int ctmi_kv_attend(const void* q, int32_t dtype, int64_t q_token_stri
   CTMI_REQUIRE(tokens >= 0 && requests >= 0 && width >= 0 && table_stride >= width, CTMI_ERR_VALUE,
                "bad sizes: %lld tokens, %lld requests, %lld table columns, stride %lld", (long long)tokens,
                (long long)requests, (long long)width, (long long)table_stride);
-  CTMI_REQUIRE(tokens < (1ll << 31) / q_heads && requests < (1ll << 31) &&
+  CTMI_REQUIRE(tokens < (1ll << 30) / q_heads && requests < (1ll << 30) &&
                    width < (1ll << 30) / blocks->block_size,
-               CTMI_ERR_UNSUPPORTED, "tokens x heads and requests must stay below 2^31, positions below 2^30");
+               CTMI_ERR_UNSUPPORTED, "tokens x heads, requests and positions must stay below 2^30");
   CTMI_REQUIRE(query_start != nullptr || tokens == requests, CTMI_ERR_VALUE,
                "without query_start every request has one token: got %lld tokens for %lld requests",
                (long long)tokens, (long long)requests);

@@ -758,10 +758,12 @@ typedef struct ctmi_kv_blocks {
 } ctmi_kv_blocks;
 
 /* Write new tokens.  key / value: [tokens, kv_heads, head_dim] of `dtype` (bf16 or f16),
- * strides in elements (head_dim contiguous).  slots: int64 [tokens], block * block_size +
- * position, tokens of one block next to each other in rising order (what ctmi_kv_plan
- * writes); a slot outside the pool (-1) skips its token.  A slot named twice in one call is
- * the caller's mistake: the block it names then holds either token's codes.
+ * strides in elements (head_dim contiguous; multiples of 8, tokens below 2^22 apart; both
+ * tensors 16-byte aligned), the pool of fewer than 2^31 slots.  slots: int64 [tokens],
+ * block * block_size + position, tokens of one block next to each other in rising order (what
+ * ctmi_kv_plan writes); a slot outside the pool (-1) skips its token.  A slot named twice in
+ * one call is the caller's mistake: the block it names then holds either token's codes, under
+ * either's scale.
  * dynamic != 0: with A = max|x| over the finite new values of a block and head, the scale
  * becomes max(A / q, eps), or the maximum of that and the scale it had unless the block's
  * first position is among the new ones; q = 448 (e4m3) or 127.5 (int8), eps = 2^-23.  Codes

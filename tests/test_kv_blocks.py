@@ -366,6 +366,12 @@ def test_plan_of_steps_that_do_not_fit(gpu):
     run_plan(gpu, [20, 3], [0, 0], table, [3, 4], 2, 16, 0)
     run_plan(gpu, [0, 0], [0, -1], table, [], 0, 16, 0)
     run_plan(gpu, [32, 3], [-1, 20], table, [3, 4, 9, 9], 0, 16, 20)  # blocks of the ended request are used again
+    from compressed_tensors_amd.modeling import plan_kv_blocks
+
+    none = torch.zeros(0, dtype=torch.int32, device=gpu)
+    plan = plan_kv_blocks(none, none, none.view(0, 2), none + 1, torch.zeros(1, dtype=torch.int32, device=gpu),
+                          block_size=16, total_tokens=3)
+    assert plan.query_start.tolist() == [0] and plan.slots.tolist() == [-1] * 3 and plan.status.tolist() == [0]
 
 
 # ---------------------------------------------------------------------------- the run of all
