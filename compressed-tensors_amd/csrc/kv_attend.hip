@@ -110,6 +110,9 @@ __device__ __forceinline__ void widen4(uint32_t w, uint32_t* o) {
 struct Operand {
   uint32_t w[4];
 };
+struct Operands {  // of 16 elements
+  Operand half[2];
+};
 
 template <typename T, bool FP8>
 __device__ __forceinline__ Operand widen8(uint32_t lo, uint32_t hi) {
@@ -142,6 +145,16 @@ __device__ __forceinline__ float groups_sum(float v) {
 // bytes of w that hold an e4m3 NaN (0x7F or 0xFF), as 0xFF each
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
   return (((w & 0x7F7F7F7Fu) + 0x01010101u) >> 7 & 0x01010101u) * 0xFFu;
+}
+
+// half `u` of 16 elements that are codes, or operands already
+template <typename T, bool FP8>
+__device__ __forceinline__ Operand operand(const Vec<uint32_t, 4>& codes, int u) {
+  return widen8<T, FP8>(codes.v[2 * u], codes.v[2 * u + 1]);
+}
+template <typename T, bool FP8>
+__device__ __forceinline__ Operand operand(const Operands& ready, int u) {
+  return ready.half[u];
 }
 
 // The rows of a wavefront and what they have gathered: RT tiles of 16, row `first` + 16 t + c
@@ -187,14 +200,14 @@ struct AttendRows {
     const int at16 = kb + (lane_id() >> 4) * 16;  // first of this lane's 16 keys
     // a step that every row sees whole, of blocks that are all there, needs no masks
     const bool whole = kb + kStep <= seen_by_all && __all(valid && ks >= 0.0f);
-    // values at keys that no row sees: whatever is there, its weight is 0 and must stay so
+    // e4m3 values at keys that no row sees: whatever is there, their weight is 0 and must stay so
     const int seen = valid ? min(max(seen_by_any - at16, 0), 16) : 0;
     auto clean = [&](Vec<uint32_t, 4> v, bool nans) {
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         const int n = min(max(seen - w * 4, 0), 4);
         v.v[w] &= n == 4 ? 0xFFFFFFFFu : (1u << (8 * n)) - 1u;
-        if (FP8 && nans) v.v[w] &= ~nan_bytes(v.v[w]);
+        if (nans) v.v[w] &= ~nan_bytes(v.v[w]);
       }
       return v;
     };
@@ -223,8 +236,8 @@ struct AttendRows {
       for (int t = 0; t < RT; ++t) s[t][kt] = f32x4{0, 0, 0, 0};
 #pragma unroll
       for (int ch = 0; ch < CH; ++ch) {
-        const Vec<uint32_t, 4> w = key(kt, ch);
-        const Operand k0 = widen8<T, FP8>(w.v[0], w.v[1]), k1 = widen8<T, FP8>(w.v[2], w.v[3]);
+        const auto w = key(kt, ch);
+        const Operand k0 = operand<T, FP8>(w, 0), k1 = operand<T, FP8>(w, 1);
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
           s[t][kt] = product<T>(k0, q[t][ch][0], s[t][kt]);
@@ -315,8 +328,12 @@ struct AttendRows {
     }
     // (two loops: a branch for each d would leave each load of a value alone with its wait)
     __builtin_amdgcn_s_setprio(1);
-    if (whole) gather(hi, lo, value);
-    else gather(hi, lo, [&](int d) { return clean(value(d), true); });
+    if constexpr (FP8) {
+      if (whole) gather(hi, lo, value);
+      else gather(hi, lo, [&](int d) { return clean(value(d), true); });
+    } else {
+      gather(hi, lo, value);
+    }
     __builtin_amdgcn_s_setprio(0);
   }
 
@@ -324,10 +341,10 @@ struct AttendRows {
   __device__ __forceinline__ void gather(const Operand (*hi)[2], const Operand (*lo)[2], Value value) {
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
-      const Vec<uint32_t, 4> w = value(d);
+      const auto w = value(d);
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const Operand v = widen8<BF16, FP8>(w.v[2 * u], w.v[2 * u + 1]);
+        const Operand v = operand<BF16, FP8>(w, u);
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
           o[t][d] = product<BF16>(v, hi[t][u], o[t][d]);
@@ -542,9 +559,22 @@ __global__ __launch_bounds__(kAttendWaves* kWave, D == 256 ? 1 : 2) void kv_atte
   const Request rq = request_of(a, r);
   const int rows = rq.queries * share;
   const int64_t bytes = (int64_t)a.block_size * D;
-  __shared__ Vec<uint32_t, 4> keys[2][kStep * KP], values[2][D * 4];
-  auto key_place = [](int key, int piece) { return key * KP + (piece ^ (((key & 3) | ((key >> 4) & 1) << 2) & (KP - 1))); };
-  auto value_place = [](int d, int group) { return d * 4 + (group ^ ((d >> 2) & 3)); };
+  // e4m3 codes stay codes in LDS: one instruction makes two elements of them.  int8 codes take
+  // more and are widened on the way in, once for the workgroup (269 against 316 us for the two
+  // prompts above; e4m3 266 against 259 that way).  Places count 16 bytes.
+  constexpr int PER = FP8 ? 1 : 2;
+  __shared__ Vec<uint32_t, 4> keys[2][kStep * KP * PER], values[2][D * 4 * PER];
+  auto key_place = [](int key, int piece) {
+    return key * KP * PER + (piece ^ (((key & 3) | ((key >> 4) & 1) << 2) & (KP * PER - 1)));
+  };
+  auto value_place = [](int d, int piece) { return d * 4 * PER + (piece ^ (FP8 ? (d >> 2) & 3 : d & 7)); };
+  auto take = [](const Vec<uint32_t, 4>* at, auto place) {  // 16 elements, place(i): their i-th 16 bytes
+    if constexpr (FP8) {
+      return at[place(0)];
+    } else {
+      return Operands{{__builtin_bit_cast(Operand, at[place(0)]), __builtin_bit_cast(Operand, at[place(1)])}};
+    }
+  };
 
   for (int tile = unit.tile; tile * ROWS < rows; tile += a.tiles) {
     const int row0 = tile * ROWS, tile_end = last_key(rq, min(row0 + ROWS, rows) - 1, share);
@@ -559,7 +589,7 @@ __global__ __launch_bounds__(kAttendWaves* kWave, D == 256 ? 1 : 2) void kv_atte
 
     Vec<uint32_t, 4> kr[PIECES], vr[PIECES];
     float ks = 0.0f, vs = 0.0f;
-    int bk[PIECES], ak[PIECES], bv, av, bs_next = 0;  // blocks of the step to load; bs: of this lane's 16 keys
+    int bk[PIECES], ak[PIECES], bv, av, bs_next = 0;  // blocks of the step to load; bs_next: of this lane's 16 keys
     const int my_key = threadIdx.x / KP, my_piece = threadIdx.x % KP, my_group = threadIdx.x % 4, my_d = threadIdx.x / 4;
     auto find = [&](int kb) {
       if constexpr (WIDE) {
@@ -603,8 +633,18 @@ __global__ __launch_bounds__(kAttendWaves* kWave, D == 256 ? 1 : 2) void kv_atte
     auto store = [&](int half) {
 #pragma unroll
       for (int p = 0; p < PIECES; ++p) {
-        keys[half][key_place(my_key + p * KEYS, my_piece)] = kr[p];
-        values[half][value_place(my_d + p * 64, my_group)] = vr[p];
+        const int key = my_key + p * KEYS, d = my_d + p * 64;
+        if constexpr (FP8) {
+          keys[half][key_place(key, my_piece)] = kr[p];
+          values[half][value_place(d, my_group)] = vr[p];
+        } else {
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            using Bits = Vec<uint32_t, 4>;
+            keys[half][key_place(key, my_piece * 2 + u)] = __builtin_bit_cast(Bits, operand<T, FP8>(kr[p], u));
+            values[half][value_place(d, my_group * 2 + u)] = __builtin_bit_cast(Bits, operand<BF16, FP8>(vr[p], u));
+          }
+        }
       }
     };
     __syncthreads();  // the tile before may still be read
@@ -625,8 +665,12 @@ __global__ __launch_bounds__(kAttendWaves* kWave, D == 256 ? 1 : 2) void kv_atte
       }
       if (kb < w.seen_by_any)
         w.step(kb, ks_now, vs_now, valid,
-               [&](int t, int ch) { return keys[half][key_place((c >> 2) * 16 + t * 4 + (c & 3), ch * 4 + j)]; },
-               [&](int d) { return values[half][value_place(d * 16 + c, j)]; }, [] {});
+               [&](int t, int ch) {
+                 const int key = (c >> 2) * 16 + t * 4 + (c & 3);
+                 return take(keys[half], [&](int i) { return key_place(key, (ch * 4 + j) * PER + i); });
+               },
+               [&](int d) { return take(values[half], [&](int i) { return value_place(d * 16 + c, j * PER + i); }); },
+               [] {});
       if (more) store(half ^ 1);
       __syncthreads();
     }
