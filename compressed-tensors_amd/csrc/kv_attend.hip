@@ -761,6 +761,7 @@ struct Launch {
   bool split_keys;
   int row_tiles, tile_rows;
   int64_t tiles, chunks, chunk_keys;
+  int64_t most_chunks;  // of any shorter max_seq, too
 };
 
 Launch plan_launch(int64_t requests, int32_t q_heads, int32_t kv_heads, int32_t head_dim, int64_t max_query,
@@ -783,8 +784,11 @@ Launch plan_launch(int64_t requests, int32_t q_heads, int32_t kv_heads, int32_t 
   if (keys < kFloor) keys = kFloor;
   l.chunk_keys = chunks == 1 && !l.split_keys ? 1 << 30 : keys;
   // requests of very different lengths: the long ones are cut further
-  if (l.split_keys && l.chunk_keys > 8192) l.chunk_keys = 8192;
+  constexpr int64_t kLongest = 8192;
+  if (l.split_keys && l.chunk_keys > kLongest) l.chunk_keys = kLongest;
   l.chunks = cdiv(max_seq, l.chunk_keys);
+  l.most_chunks = cdiv(max_seq, kFloor) < chunks ? cdiv(max_seq, kFloor) : chunks;
+  if (l.split_keys && cdiv(max_seq, kLongest) > l.most_chunks) l.most_chunks = cdiv(max_seq, kLongest);
   return l;
 }
 
@@ -797,8 +801,10 @@ extern "C" int64_t ctmi_kv_attend_tmp_bytes(int64_t tokens, int64_t requests, in
                                             int32_t kv_heads, int32_t head_dim, int64_t max_query,
                                             int64_t max_seq) {
   if (tokens < 1 || requests < 1 || q_heads < 1 || kv_heads < 1 || max_query < 1 || max_seq < 1) return 0;
+  if (max_query > tokens) max_query = tokens;
+  if (max_seq > 1ll << 30) max_seq = 1ll << 30;
   const Launch l = plan_launch(requests, q_heads, kv_heads, head_dim, max_query, max_seq);
-  return l.chunks > 1 ? l.chunks * tokens * q_heads * (head_dim + 2) * 4 : 0;
+  return l.most_chunks > 1 ? l.most_chunks * tokens * q_heads * (head_dim + 2) * 4 : 0;
 }
 
 extern "C" int ctmi_kv_attend(const void* q, int32_t dtype, int64_t q_token_stride, int64_t q_head_stride,

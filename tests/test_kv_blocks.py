@@ -12,6 +12,8 @@ are divided by the sum of the rounded weights, w' = w (1 + d) with |d| <= e, the
 sum p (1 + d) v / sum p (1 + d): off by at most e sum p |v| above and, through the sum below,
 by e / (1 - e) |o| once more.  The output's rounding is eps / 2 of the value.
 """
+import ctypes
+
 import pytest
 import torch
 
@@ -182,6 +184,29 @@ def test_nothing_leaks_from_positions_that_are_hidden(gpu, codes, news):
                                           cache[2], cache[3])], table, lens_t, starts)
         off = (got.double() - want).abs()[clean]
         assert (off <= 2.0 ** -7 * mag[clean] + 1e-6).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("max_query,max_seq", [(1, 1), (7, 1 << 20), (1 << 40, 4097), (1000, 1 << 40)])
+def test_any_launch_hint_has_room_in_the_scratch_it_is_given(gpu, ctmi, max_query, max_seq):
+    """hints beyond the tokens and the table are cut to them by the call, which may then split
+    the keys otherwise than the hints alone would"""
+    from compressed_tensors_amd import _lib
+    from compressed_tensors_amd.modeling import KVBlocks
+    from compressed_tensors_amd.modeling.kv_blocks import _describe
+
+    announce("hints", max_query, max_seq)
+    q, cache, table, lens, starts = attention_case([1500, 2049], [5, 2], 8, 2, 64, 64, FP8, torch.bfloat16)
+    on = KVBlocks(*(t.to(gpu) for t in cache))
+    c, qd, td, ld, sd = _describe(on), q.to(gpu), table.to(gpu), lens.to(gpu), starts.to(gpu)
+    out = torch.full_like(qd, 7.0)
+    size = ctmi.ctmi_kv_attend_tmp_bytes(7, 2, 8, 2, 64, max_query, max_seq)
+    tmp = torch.empty(size + 16, dtype=torch.uint8, device=gpu)
+    _lib.check(ctmi.ctmi_kv_attend(
+        qd.data_ptr(), _lib.dtype_code(q.dtype), 512, 64, out.data_ptr(), 7, 8, ctypes.byref(c), td.data_ptr(),
+        td.shape[1], td.shape[1], ld.data_ptr(), sd.data_ptr(), 2, 0.125, max_query, max_seq, tmp.data_ptr(), size,
+        _lib.stream_of(qd.device)))
+    check_attention(out, q, cache, table, lens, starts)
 
 
 @pytest.mark.gpu
