@@ -208,6 +208,21 @@ def test_compressed_linear_that_keeps_its_weight_packed(gpu, dtype, symmetric, s
     assert module.quantization_status == QuantizationStatus.COMPRESSED and not hasattr(module, "weight")
 
 
+@pytest.mark.gpu
+def test_keep_packed_with_other_types_of_scales_and_inputs(gpu):
+    """any number of rows takes what few rows take; inputs of 32 bits go through the decompressed weight"""
+    announce("keep_packed, other types")
+    module, packed, scale, zero, b = packed_module(gpu, torch.bfloat16, True, "group", bias=False)
+    module.weight_scale.data = module.weight_scale.data.float()
+    dense = module.compressor.decompress_module(module)
+    with torch.no_grad():
+        x = torch.randn(193, 256).to(torch.bfloat16)
+        check(module(x[:7].to(gpu)), x[:7], packed, scale, zero, b)
+        assert torch.equal(module(x.to(gpu)), torch.nn.functional.linear(x.to(gpu), dense.to(x.dtype)))
+        x = torch.randn(3, 256).to(gpu)
+        assert torch.equal(module(x), torch.nn.functional.linear(x, dense.float()))
+
+
 def test_keep_packed_refusals():
     from compressed_tensors_amd import CompressedLinear
     from compressed_tensors_amd.quantization import QuantizationArgs, QuantizationScheme
