@@ -197,6 +197,16 @@ struct AttendRows {
     }
   }
 
+  // the queries are there: not to be waited for behind the loads of a step
+  __device__ __forceinline__ void arrived() {
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+      for (int ch = 0; ch < CH; ++ch)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) asm volatile("" : "+v"(q[t][ch][i / 4].w[i % 4]));
+  }
+
   // 64 keys from kb on.  key(t, ch): 16 bytes of this lane's row of key tile t; value(d): the
   // codes of its 16 keys in dimension d * 16 + c.  ks, vs: the scales of those keys' block (ks
   // with the softmax's); valid: whether there is one.  keys_done() comes when the last key is used.
@@ -409,11 +419,11 @@ struct AttendUnit {
 };
 
 // the block of 16 keys from `key` on, and where in it they start
-__device__ __forceinline__ int look_up(const AttendArgs& a, int r, int key, int* at) {
+__device__ __forceinline__ int look_up(const AttendArgs& a, int r, int key, int* at, uint32_t nothing = 0) {
   const uint32_t u = (uint32_t)key >> 4;
   const uint32_t index = a.magic ? __umulhi(u, a.magic) : u;
   *at = (int)(u - index * a.sixteenths) * 16;
-  return a.table[(int64_t)r * a.table_stride + min((int)index, a.width - 1)];
+  return (a.table + (int64_t)r * a.table_stride + min((int)index, a.width - 1))[nothing];
 }
 __device__ __forceinline__ bool in_pool(const AttendArgs& a, int block) { return (uint32_t)block < (uint32_t)a.num_blocks; }
 __device__ __forceinline__ int64_t cell_of(const AttendArgs& a, int block, int kv) {
@@ -449,7 +459,7 @@ __global__ __launch_bounds__(kAttendWaves* kWave, D == 256 || RT == 2 ? 1 : 2) v
     constexpr int STRIDE = kAttendWaves * kStep;
     Vec<uint32_t, 4> kw[4][CH], vw[DT];
     float ks = 0.0f, vs = 0.0f;
-    int bk = 0, ak = 0, bv = 0, av = 0;  // block and position: of the keys this lane multiplies, of those it gets
+    int bk, ak, bv, av;  // block and position: of the keys this lane multiplies, of those it gets
     auto load_keys = [&](int block, int at) {
       const uint8_t* p = a.key + cell_of(a, block, kv) * bytes + (at + (c & 3)) * D + j * 16;
 #pragma unroll
@@ -466,29 +476,35 @@ __global__ __launch_bounds__(kAttendWaves* kWave, D == 256 || RT == 2 ? 1 : 2) v
 #pragma unroll
       for (int d = 0; d < DT; ++d) vw[d] = ldg_nt<uint32_t, 4>((const uint32_t*)(p + d * 16 * a.block_size));
     };
+    // What a step multiplies is asked for one step before it, where its blocks lie two steps
+    // before: no address waits for a load that others were asked for ahead of.  Behind the last
+    // step that one comes again, from the cache: a branch around the loads, or around the loop,
+    // would make each wait in it one for all of them (6 requests of up to 32768: 91 us so, 83 now).
     if (key0 < key1) {
+      const int last = key0 + (key1 - 1 - key0) / STRIDE * STRIDE;
       bk = look_up(a, r, key0 + (c >> 2) * 16, &ak);
       bv = look_up(a, r, key0 + j * 16, &av);
+      const int second = min(key0 + STRIDE, last);
       load_keys(bk, ak);
+      bk = look_up(a, r, second + (c >> 2) * 16, &ak);
       load_scales(bv);
       load_values(bv, av);
-    }
-    for (int kb = key0; kb < key1; kb += STRIDE) {
-      const bool more = kb + STRIDE < key1;
-      const bool valid = in_pool(a, bv);
-      const float ks_now = ks * a.scale, vs_now = vs;
-      if (more) {
-        bk = look_up(a, r, kb + STRIDE + (c >> 2) * 16, &ak);
-        bv = look_up(a, r, kb + STRIDE + j * 16, &av);
-      }
-      w.step(kb, ks_now, vs_now, valid, [&](int t, int ch) { return kw[t][ch]; }, [&](int d) { return vw[d]; },
-             [&] {
-               if (more) {
+      int bs = bv;  // block of the scales
+      bv = look_up(a, r, second + j * 16, &av);
+      for (int kb = key0; kb < key1; kb += STRIDE) {
+        const bool valid = in_pool(a, bs);
+        const float ks_now = ks * a.scale, vs_now = vs;
+        const int later = min(kb + 2 * STRIDE, last);
+        w.step(kb, ks_now, vs_now, valid, [&](int t, int ch) { return kw[t][ch]; }, [&](int d) { return vw[d]; },
+               [&] {
                  load_keys(bk, ak);
-                 load_scales(bv);
-               }
-             });
-      if (more) load_values(bv, av);
+                 bk = look_up(a, r, later + (c >> 2) * 16, &ak);
+               });
+        load_scales(bv);
+        load_values(bv, av);
+        bs = bv;
+        bv = look_up(a, r, later + j * 16, &av);
+      }
     }
     w.finish();
 
@@ -596,9 +612,11 @@ __global__ __launch_bounds__(kAttendWaves* kWave, D == 256 ? 1 : 2) void kv_atte
     float ks = 0.0f, vs = 0.0f;
     int bk[PIECES], ak[PIECES], bv, av, bs_next = 0;  // blocks of the step to load; bs_next: of this lane's 16 keys
     const int my_key = threadIdx.x / KP, my_piece = threadIdx.x % KP, my_group = threadIdx.x % 4, my_d = threadIdx.x / 4;
+    uint32_t nothing = 0;  // which only the lanes know: what is read with it stays theirs until found()
+    asm volatile("" : "+v"(nothing));
     auto find = [&](int kb) {
       if constexpr (WIDE) {
-        bv = __builtin_amdgcn_readfirstlane(look_up(a, r, __builtin_amdgcn_readfirstlane(kb), &av));
+        bv = look_up(a, r, __builtin_amdgcn_readfirstlane(kb), &av, nothing);
         av = __builtin_amdgcn_readfirstlane(av);
       } else {
 #pragma unroll
@@ -609,6 +627,12 @@ __global__ __launch_bounds__(kAttendWaves* kWave, D == 256 ? 1 : 2) void kv_atte
         }
         bv = look_up(a, r, kb + my_group * 16, &av);
       }
+    };
+    // What find and load ask for is first looked at when a step is over: a number made uniform or
+    // multiplied where it is asked for would hold the step up until it is there, with all that
+    // was asked for before it (blocks of 16: 277 us so, 258 now; 64 dimensions 181 and 165).
+    auto found = [&] {
+      if constexpr (WIDE) bv = __builtin_amdgcn_readfirstlane(bv);
     };
     const uint32_t key_at = threadIdx.x * 16, value_at = my_d * a.block_size + my_group * 16, value_step = 64 * a.block_size;
     auto load = [&] {
@@ -621,7 +645,7 @@ __global__ __launch_bounds__(kAttendWaves* kWave, D == 256 ? 1 : 2) void kv_atte
           vr[p] = ldg<uint32_t, 4>((const uint32_t*)(v + (value_at + p * value_step)));
         }
         bs_next = bv;
-        ks = a.key_scale[cell] * a.scale;
+        ks = a.key_scale[cell];
         vs = a.value_scale[cell];
       } else {
 #pragma unroll
@@ -631,7 +655,7 @@ __global__ __launch_bounds__(kAttendWaves* kWave, D == 256 ? 1 : 2) void kv_atte
 #pragma unroll
         for (int p = 0; p < PIECES; ++p) vr[p] = ldg<uint32_t, 4>((const uint32_t*)(v + p * value_step));
         bs_next = __shfl(bv, j, kWave);  // lane j's group is j
-        ks = a.key_scale[cell_of(a, bs_next, kv)] * a.scale;
+        ks = a.key_scale[cell_of(a, bs_next, kv)];
         vs = a.value_scale[cell_of(a, bs_next, kv)];
       }
     };
@@ -655,19 +679,20 @@ __global__ __launch_bounds__(kAttendWaves* kWave, D == 256 ? 1 : 2) void kv_atte
     __syncthreads();  // the tile before may still be read
     if (key0 < key1) {
       find(key0);
+      found();
       load();
       find(key0 + kStep);
       store(0);
+      found();
     }
     __syncthreads();
+    w.arrived();
     int half = 0;
     for (int kb = key0; kb < key1; kb += kStep, half ^= 1) {
-      const float ks_now = ks, vs_now = vs;
-      const bool valid = in_pool(a, bs_next), more = kb + kStep < key1;
-      if (more) {
-        load();
-        find(kb + 2 * kStep);
-      }
+      const float ks_now = ks * a.scale, vs_now = vs;
+      const bool valid = in_pool(a, bs_next);
+      load();  // behind the last step, too: the table's last block, or the pool's first
+      find(kb + 2 * kStep);
       if (kb < w.seen_by_any)
         w.step(kb, ks_now, vs_now, valid,
                [&](int t, int ch) {
@@ -676,7 +701,8 @@ __global__ __launch_bounds__(kAttendWaves* kWave, D == 256 ? 1 : 2) void kv_atte
                },
                [&](int d) { return take(values[half], [&](int i) { return value_place(d * 16 + c, j * PER + i); }); },
                [] {});
-      if (more) store(half ^ 1);
+      store(half ^ 1);
+      found();
       __syncthreads();
     }
     w.finish();
