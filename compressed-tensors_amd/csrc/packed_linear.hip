@@ -24,6 +24,8 @@
 // Measured on one MI355X (groups of 128): 1 x 4096 x 4096 5.7 us, of which the bytes are 1.7;
 // 16 x 28672 x 4096 21 us, 3.0 TB/s, with the vector units 28 % busy - 5.7 us of ramp are in
 // it, whatever the size; 64 x 4096 x 14336 23 us and 4.6 us for the sum of its parts.
+#include <type_traits>
+
 #include "ctmi_device.h"
 #include "ctmi_host.h"
 
@@ -31,6 +33,7 @@ namespace ctmi {
 namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
@@ -96,11 +99,11 @@ __device__ __forceinline__ Operand signed_codes_of(uint32_t w, float zero) {
 
 // The four lane groups hold words 4 j + t; afterwards w[t] is word 4 t + j: 32 neighbouring
 // columns per product.
-__device__ __forceinline__ void transpose4(uint32_t* w) {
+__device__ __forceinline__ void transpose4(const u32x4& from, uint32_t* w) {
   typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 #pragma unroll
   for (int t = 0; t < 4; t += 2) {
-    const u32x2 r = __builtin_amdgcn_permlane16_swap(w[t], w[t + 1], false, false);
+    const u32x2 r = __builtin_amdgcn_permlane16_swap(from[t], from[t + 1], false, false);
     w[t] = r[0], w[t + 1] = r[1];
   }
 #pragma unroll
@@ -115,13 +118,20 @@ __device__ __forceinline__ void transpose4(uint32_t* w) {
 constexpr uint32_t kNowhere = 0x80000000u;
 struct Buffer {
   __amdgpu_buffer_rsrc_t r;
+  // (a descriptor whose numbers the compiler has put into lanes is looked at lane by lane, in a
+  // loop around each load)
+  static __device__ __forceinline__ void* uniform(const void* p) {
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)p);
+    const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)((uintptr_t)p >> 32));
+    return (void*)((uintptr_t)hi << 32 | lo);
+  }
   __device__ __forceinline__ Buffer(const void* base, uint32_t bytes)
-      : r(__builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)bytes, 0x00027000)) {}
+      : r(__builtin_amdgcn_make_buffer_rsrc(uniform(base), 0, __builtin_amdgcn_readfirstlane((int)bytes), 0x00027000)) {}
   __device__ __forceinline__ Vec<uint32_t, 4> load16(uint32_t at) const {
     return __builtin_bit_cast(Vec<uint32_t, 4>, __builtin_amdgcn_raw_buffer_load_b128(r, (int)at, 0, 0));
   }
   __device__ __forceinline__ uint32_t load4(uint32_t at) const { return __builtin_amdgcn_raw_buffer_load_b32(r, (int)at, 0, 0); }
-  __device__ __forceinline__ uint32_t load2(uint32_t at) const { return __builtin_amdgcn_raw_buffer_load_b16(r, (int)at, 0, 0); }
+  __device__ __forceinline__ uint16_t load2(uint32_t at) const { return __builtin_amdgcn_raw_buffer_load_b16(r, (int)at, 0, 0); }
 };
 
 // SMALL: groups that are no multiple of 128 columns, so a scale holds for one product of 32
@@ -146,8 +156,11 @@ template <typename T, int MT, int NT, int XL, bool SMALL, bool WIDE>
 struct LinearWave {
   static constexpr int PARTS = SMALL ? 4 : 1;  // groups in a step
   struct Step {
-    Vec<uint32_t, 4> w[NT];
-    uint32_t s[PARTS], z[PARTS];  // scale of weight row `lane`, zero points of rows 8 (lane % 8) on
+    u32x4 w[NT];  // (one value: a number of it carried from step to step by itself is copied there)
+    // scale of weight row `lane` (as it is stored: widened where it is asked for, it would be used
+    // there), zero points of rows 8 (lane % 8) on
+    std::conditional_t<WIDE, uint32_t, uint16_t> s[PARTS];
+    uint32_t z[PARTS];
     Vec<uint32_t, 4> x[XL];       // rows 4 i + lane / 16, columns (lane % 16) * 8 on
   };
 
@@ -201,7 +214,8 @@ struct LinearWave {
 #pragma unroll
     for (int i = 0; i < PARTS; ++i) {
       const uint32_t g = min(at.g, a.groups - 1);
-      st.s[i] = WIDE ? s_buf.load4(there ? s_at + g * 4u : kNowhere) : s_buf.load2(there ? s_at + g * 2u : kNowhere);
+      if constexpr (WIDE) st.s[i] = s_buf.load4(there ? s_at + g * 4u : kNowhere);
+      else st.s[i] = s_buf.load2(there ? s_at + g * 2u : kNowhere);
       st.z[i] = z_buf.load4(there ? z_at + g * 4u : kNowhere);
       at.left -= SMALL ? 32 : kStepK;
       const int over = (int)((uint32_t)(at.left - 1) >> 31);  // no branch here either
@@ -213,7 +227,7 @@ struct LinearWave {
     // (behind the row's end x is 0 and the codes are the next row's: they do not count)
     const uint32_t wk = there ? w_at + (uint32_t)kb / 2u : kNowhere, xk = (int)there & (int)(kb + c * 8 < a.k) ? x_at + (uint32_t)kb * 2u : kNowhere;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) st.w[t] = w_buf.load16(wk + t * w_tile);
+    for (int t = 0; t < NT; ++t) st.w[t] = __builtin_bit_cast(u32x4, w_buf.load16(wk + t * w_tile));
     load_scales(st, at, there);
 #pragma unroll
     for (int i = 0; i < XL; ++i) st.x[i] = x_buf.load16(xk + i * x_four);
@@ -225,7 +239,7 @@ struct LinearWave {
     for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        st.w[t].v[i] = w_buf.load4(kb / 8 + j * 4 + i < a.words ? w_at + kb / 2 + t * w_tile + i * 4 : kNowhere);
+        st.w[t][i] = w_buf.load4(kb / 8 + j * 4 + i < a.words ? w_at + kb / 2 + t * w_tile + i * 4 : kNowhere);
     Groups at = groups_at(kb);
     load_scales(st, at, true);
 #pragma unroll
@@ -235,7 +249,7 @@ struct LinearWave {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         st.x[i].v[e] = x_buf.load2(first + 2 * e < a.k ? at + 4 * e : kNowhere) |
-                       x_buf.load2(first + 2 * e + 1 < a.k ? at + 4 * e + 2 : kNowhere) << 16;
+                       (uint32_t)x_buf.load2(first + 2 * e + 1 < a.k ? at + 4 * e + 2 : kNowhere) << 16;
     }
   }
 
@@ -252,7 +266,7 @@ struct LinearWave {
       for (int t = 0; t < 4; ++t) x[mt][t] = __builtin_bit_cast(Operand, mine[(mt * 16 + c) * 16 + ((t * 4 + j) ^ c)]);
     auto add = [&](f32x4 sum, const Operand& v) { return product<T>(v, ones, sum); };
     auto scale_zero = [&](int nt, int part, float& s, float& z) {
-      const uint32_t raw = __shfl(st.s[part], nt * 16 + c, kWave), zeros = __shfl(st.z[part], nt * 2 + (c >> 3), kWave);
+      const uint32_t raw = __shfl((uint32_t)st.s[part], nt * 16 + c, kWave), zeros = __shfl(st.z[part], nt * 2 + (c >> 3), kWave);
       s = WIDE ? u2f(raw) : T::to_f32((uint16_t)raw);
       z = (float)(((zeros >> (4 * (c & 7))) & 15u) | z_none);
     };
@@ -260,8 +274,9 @@ struct LinearWave {
 #pragma unroll
       for (int i = 0; i < 4; ++i) y[nt][mt][i] = fmaf(s, SIGNED ? acc[i] : fmaf(-z, sum[i], acc[i]), y[nt][mt][i]);
     };
+    uint32_t codes[NT][4];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) transpose4(st.w[nt].v);
+    for (int nt = 0; nt < NT; ++nt) transpose4(st.w[nt], codes[nt]);
     f32x4 sums[MT];
     if constexpr (SMALL) {
 #pragma unroll
@@ -272,7 +287,7 @@ struct LinearWave {
         for (int nt = 0; nt < NT; ++nt) {
           float s, z;
           scale_zero(nt, t, s, z);
-          const Operand w = SIGNED ? signed_codes_of<T>(st.w[nt].v[t], z) : codes_of<T>(st.w[nt].v[t]);
+          const Operand w = SIGNED ? signed_codes_of<T>(codes[nt][t], z) : codes_of<T>(codes[nt][t]);
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt) take(nt, mt, s, z, product<T>(x[mt][t], w, f32x4{0, 0, 0, 0}), sums[mt]);
         }
@@ -295,7 +310,7 @@ struct LinearWave {
         for (int mt = 0; mt < MT; ++mt) acc[mt] = f32x4{0, 0, 0, 0};
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-          const Operand w = SIGNED ? signed_codes_of<T>(st.w[nt].v[t], z) : codes_of<T>(st.w[nt].v[t]);
+          const Operand w = SIGNED ? signed_codes_of<T>(codes[nt][t], z) : codes_of<T>(codes[nt][t]);
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt) acc[mt] = product<T>(x[mt][t], w, acc[mt]);
         }
@@ -343,7 +358,7 @@ __global__ __launch_bounds__(WAVES* kWave, PER_SIMD) void packed_linear_kernel(L
   // each wavefront's x, TM rows of 256 bytes; at the end [wave][TM][TN] sums
   extern __shared__ Vec<uint32_t, 4> lds[];
   float* meet = (float*)lds;
-  const int wave = threadIdx.x / kWave, waves = blockDim.x / kWave;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), waves = blockDim.x / kWave;
   const int n0 = blockIdx.x * TN;
   LinearWave<T, MT, NT, XL, SMALL, WIDE> w(a, n0, blockIdx.y * TM, lds + wave * TM * 16);
   const int64_t begin = ((int64_t)blockIdx.z * waves + wave) * a.wave_k;
@@ -390,8 +405,9 @@ template <typename T, int MT, int NT, bool SMALL, bool WIDE>
 struct LinearShared {
   static constexpr int PARTS = SMALL ? 4 : 1, ACROSS = 4, ALONG = 2;
   struct Step {
-    Vec<uint32_t, 4> w[NT];
-    uint32_t s[PARTS], z[PARTS];
+    u32x4 w[NT];
+    std::conditional_t<WIDE, uint32_t, uint16_t> s[PARTS];
+    uint32_t z[PARTS];
   };
   const LinearArgs& a;
   int lane, c, j;
@@ -437,11 +453,12 @@ struct LinearShared {
   __device__ __forceinline__ void load(Step& st, int kb, bool there, Groups& at) const {
     const uint32_t wk = there ? w_at + (uint32_t)kb / 2u : kNowhere;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) st.w[t] = w_buf.load16(wk + t * w_tile);
+    for (int t = 0; t < NT; ++t) st.w[t] = __builtin_bit_cast(u32x4, w_buf.load16(wk + t * w_tile));
 #pragma unroll
     for (int i = 0; i < PARTS; ++i) {
       const uint32_t g = min(at.g, a.groups - 1);
-      st.s[i] = WIDE ? s_buf.load4(there ? s_at + g * 4u : kNowhere) : s_buf.load2(there ? s_at + g * 2u : kNowhere);
+      if constexpr (WIDE) st.s[i] = s_buf.load4(there ? s_at + g * 4u : kNowhere);
+      else st.s[i] = s_buf.load2(there ? s_at + g * 2u : kNowhere);
       st.z[i] = z_buf.load4(there ? z_at + g * 4u : kNowhere);
       at.left -= SMALL ? 32 : kStepK;
       const int over = (int)((uint32_t)(at.left - 1) >> 31);
@@ -466,8 +483,9 @@ struct LinearShared {
   __device__ __forceinline__ void step(Step& st, X x) {
     const Operand ones = T::id == CTMI_BF16 ? Operand{{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u}}
                                             : Operand{{0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u}};
+    uint32_t codes[NT][4];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) transpose4(st.w[nt].v);
+    for (int nt = 0; nt < NT; ++nt) transpose4(st.w[nt], codes[nt]);
     f32x4 acc[NT][MT], sums[MT];
     float s[NT], z[NT];
 #pragma unroll
@@ -477,7 +495,7 @@ struct LinearShared {
         for (int mt = 0; mt < MT; ++mt) sums[mt] = f32x4{0, 0, 0, 0};
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          const uint32_t raw = __shfl(st.s[t], nt * 16 + c, kWave), zeros = __shfl(st.z[t], nt * 2 + (c >> 3), kWave);
+          const uint32_t raw = __shfl((uint32_t)st.s[t], nt * 16 + c, kWave), zeros = __shfl(st.z[t], nt * 2 + (c >> 3), kWave);
           s[nt] = WIDE ? u2f(raw) : T::to_f32((uint16_t)raw);
           z[nt] = (float)(((zeros >> (4 * (c & 7))) & 15u) | z_none);
 #pragma unroll
@@ -486,7 +504,7 @@ struct LinearShared {
       }
       Operand w[NT];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) w[nt] = SIGNED ? signed_codes_of<T>(st.w[nt].v[t], z[nt]) : codes_of<T>(st.w[nt].v[t]);
+      for (int nt = 0; nt < NT; ++nt) w[nt] = SIGNED ? signed_codes_of<T>(codes[nt][t], z[nt]) : codes_of<T>(codes[nt][t]);
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
         const Operand v = x(mt, t);
@@ -515,9 +533,11 @@ struct LinearShared {
     Groups at = groups_at(min(k0, a.k - 1));
     load_rows(rows, k0, k0 < k1);
     load(one, k0, k0 < k1, at);
+    __builtin_amdgcn_sched_barrier(0);
     store_rows(rows, lds);
     load_rows(rows, k0 + kStepK, k0 + kStepK < k1);
     load(two, k0 + kStepK, k0 + kStepK < k1, at);
+    __builtin_amdgcn_sched_barrier(0);
     __syncthreads();
     auto from = [&](const Vec<uint32_t, 4>* tile) {
       return [tile, this](int mt, int t) { return __builtin_bit_cast(Operand, tile[(mt * 16 + c) * 16 + ((t * 4 + j) ^ c)]); };
@@ -525,14 +545,18 @@ struct LinearShared {
 #pragma unroll 1
     for (int kb = k0; kb < k0 + a.wave_k; kb += 2 * kStepK) {
       step<false>(one, from(lds));
+      __builtin_amdgcn_sched_barrier(0);
       store_rows(rows, lds + TILE);
       load_rows(rows, kb + 2 * kStepK, kb + 2 * kStepK < k1);
       load(one, kb + 2 * kStepK, kb + 2 * kStepK < k1, at);
+      __builtin_amdgcn_sched_barrier(0);
       __syncthreads();
       step<false>(two, from(lds + TILE));
+      __builtin_amdgcn_sched_barrier(0);
       store_rows(rows, lds);
       load_rows(rows, kb + 3 * kStepK, kb + 3 * kStepK < k1);
       load(two, kb + 3 * kStepK, kb + 3 * kStepK < k1, at);
+      __builtin_amdgcn_sched_barrier(0);
       __syncthreads();
     }
   }
@@ -558,7 +582,7 @@ __global__ __launch_bounds__(8 * kWave, 2) void packed_linear_shared_kernel(Line
   using Wave = LinearShared<T, MT, NT, SMALL, WIDE>;
   constexpr int TM = MT * 16, TN = Wave::ACROSS * NT * 16;
   extern __shared__ Vec<uint32_t, 4> lds[];  // x: two steps for each half of k; then sums [TM][TN]
-  const int wave = threadIdx.x / kWave, across = wave % Wave::ACROSS, along = wave / Wave::ACROSS;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), across = wave % Wave::ACROSS, along = wave / Wave::ACROSS;
   const int n0 = blockIdx.x * TN, m0 = blockIdx.y * TM;
   Wave w(a, n0 + across * NT * 16, m0, across);
   const int64_t begin = ((int64_t)blockIdx.z * Wave::ALONG + along) * a.wave_k;
