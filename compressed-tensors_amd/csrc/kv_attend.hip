@@ -803,14 +803,19 @@ Launch plan_launch(int64_t requests, int32_t q_heads, int32_t kv_heads, int32_t 
   l.row_tiles = head_dim == 256 || rows <= 16 ? 1 : 2;
   l.tile_rows = (l.split_keys ? 1 : kAttendWaves) * l.row_tiles * 16;
   l.tiles = cdiv(rows, l.tile_rows);
-  // As many workgroups as are resident at once (two per compute unit), in one go: with 512 of
-  // them 64 x 4096 takes 81 to 88 us, with 768 121 and with 1024 to 2048 89 to 98.  Chunks
-  // below kFloor keys cost more to bring together than they gain.
-  constexpr int64_t kResident = 512, kFloor = 256;
+  // As many workgroups as are resident at once (two per compute unit; one, where registers
+  // leave room for one), in one go: with 512 of them 64 x 4096 takes 81 to 88 us, with 768 121 and
+  // with 1024 to 2048 89 to 98; 4 requests of 16 queries over 1500 keys 18 us with 192, with 384,
+  // one and a half times what is resident, 25.
+  constexpr int64_t kFloor = 256;
+  const int64_t resident = head_dim == 256 || (l.split_keys && l.row_tiles == 2) ? 256 : 512;
   const int64_t units = requests * kv_heads * l.tiles;
-  int64_t chunks = kResident / (units < kResident ? units : kResident);
+  int64_t chunks = resident / (units < resident ? units : resident);
   // a chunk's sums leave and come back in fp32: not for more rows than the keys they stand for
-  if (!l.split_keys && units >= kResident / 2) chunks = 1;
+  if (!l.split_keys && units >= resident / 2) chunks = 1;
+  // Bringing parts together is a launch, and costs what 1024 keys do (32 requests, 1000 keys:
+  // one workgroup each 17 us, two 21; 2000 keys 26 and 33; one request, 2000 keys: 16, eight 11)
+  if (l.split_keys && max_seq * (chunks - 1) <= 1024 * chunks) chunks = 1;
   int64_t keys = cdiv(cdiv(max_seq, chunks), 256) * 256;
   if (keys < kFloor) keys = kFloor;
   l.chunk_keys = chunks == 1 && !l.split_keys ? 1 << 30 : keys;
