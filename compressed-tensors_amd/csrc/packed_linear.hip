@@ -21,9 +21,9 @@
 // The wavefronts of a workgroup, and workgroups along grid z, split k; sums meet in LDS and,
 // for a split over workgroups, in a second kernel.
 //
-// Measured on one MI355X (groups of 128): 1 x 4096 x 4096 5.7 us, of which the bytes are 1.7;
-// 16 x 28672 x 4096 21 us, 3.0 TB/s, with the vector units 28 % busy - 5.7 us of ramp are in
-// it, whatever the size; 64 x 4096 x 14336 23 us and 4.6 us for the sum of its parts.
+// Measured on one MI355X (groups of 128): 1 x 4096 x 4096 5.6 us, of which the bytes are 1.7;
+// 16 x 28672 x 4096 20 us, 3.2 TB/s, with the vector units 27 % busy - 5.6 us of ramp are in
+// it, whatever the size; 64 x 4096 x 14336 21 us and 4.8 us for the sum of its parts.
 #include <type_traits>
 
 #include "ctmi_device.h"
