@@ -460,8 +460,9 @@ __global__ __launch_bounds__(kAttendWaves* kWave, D == 256 || RT == 2 ? 1 : 2) v
     Vec<uint32_t, 4> kw[4][CH], vw[DT];
     float ks = 0.0f, vs = 0.0f;
     int bk, ak, bv, av;  // block and position: of the keys this lane multiplies, of those it gets
-    auto load_keys = [&](int block, int at) {
-      const uint8_t* p = a.key + cell_of(a, block, kv) * bytes + (at + (c & 3)) * D + j * 16;
+    // (not there: all lanes read the pool's first block, the same few lines for every wavefront)
+    auto load_keys = [&](int block, int at, bool there) {
+      const uint8_t* p = a.key + (there ? cell_of(a, block, kv) * bytes + (at + (c & 3)) * D + j * 16 : 0);
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -471,37 +472,39 @@ __global__ __launch_bounds__(kAttendWaves* kWave, D == 256 || RT == 2 ? 1 : 2) v
       ks = a.key_scale[cell_of(a, block, kv)];
       vs = a.value_scale[cell_of(a, block, kv)];
     };
-    auto load_values = [&](int block, int at) {
-      const uint8_t* p = a.value + cell_of(a, block, kv) * bytes + c * a.block_size + at;
+    auto load_values = [&](int block, int at, bool there) {
+      const uint8_t* p = a.value + (there ? cell_of(a, block, kv) * bytes + c * a.block_size + at : 0);
 #pragma unroll
       for (int d = 0; d < DT; ++d) vw[d] = ldg_nt<uint32_t, 4>((const uint32_t*)(p + d * 16 * a.block_size));
     };
     // What a step multiplies is asked for one step before it, where its blocks lie two steps
     // before: no address waits for a load that others were asked for ahead of.  Behind the last
-    // step that one comes again, from the cache: a branch around the loads, or around the loop,
-    // would make each wait in it one for all of them (6 requests of up to 32768: 91 us so, 83 now).
+    // step the loads stay, but read nothing new: a branch around them, or around the loop, would
+    // make each wait in it one for all of them (6 requests of up to 32768: 91 us so, 81 now; with
+    // the last step read again 83).
     if (key0 < key1) {
       const int last = key0 + (key1 - 1 - key0) / STRIDE * STRIDE;
       bk = look_up(a, r, key0 + (c >> 2) * 16, &ak);
       bv = look_up(a, r, key0 + j * 16, &av);
       const int second = min(key0 + STRIDE, last);
-      load_keys(bk, ak);
+      load_keys(bk, ak, true);
       bk = look_up(a, r, second + (c >> 2) * 16, &ak);
       load_scales(bv);
-      load_values(bv, av);
+      load_values(bv, av, true);
       int bs = bv;  // block of the scales
       bv = look_up(a, r, second + j * 16, &av);
       for (int kb = key0; kb < key1; kb += STRIDE) {
         const bool valid = in_pool(a, bs);
         const float ks_now = ks * a.scale, vs_now = vs;
         const int later = min(kb + 2 * STRIDE, last);
+        const bool more = kb < last;
         w.step(kb, ks_now, vs_now, valid, [&](int t, int ch) { return kw[t][ch]; }, [&](int d) { return vw[d]; },
                [&] {
-                 load_keys(bk, ak);
+                 load_keys(bk, ak, more);
                  bk = look_up(a, r, later + (c >> 2) * 16, &ak);
                });
         load_scales(bv);
-        load_values(bv, av);
+        load_values(bv, av, more);
         bs = bv;
         bv = look_up(a, r, later + j * 16, &av);
       }
