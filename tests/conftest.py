@@ -1,4 +1,5 @@
 import ctypes
+import gc
 import os
 import subprocess
 import sys
@@ -13,6 +14,14 @@ sys.path.insert(0, str(ROOT / "compressed-tensors_amd"))
 
 def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a real MI355X (run with -m gpu)")
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _nothing_left_behind():
+    """modules and graphs of a file's tests hold each other in cycles: freed here, their memory
+    does not go back to the GPU while a later file's test counts what is allocated"""
+    yield
+    gc.collect()
 
 
 def _ensure_oracle_lib() -> Path:
