@@ -5,7 +5,7 @@
 // (new tokens, blocks to take, blocks given back) for itself in LDS - at most 4096 requests,
 // 16 a thread -, then fills its share of the outputs.  Workgroups never wait for each other
 // and no output is read back, which is why inputs and outputs may not overlap.
-// Measured on one MI355X: 24 requests 7 us, 1000 requests (3.8 MB in and out) 15 us.
+// Measured on one MI355X: 24 requests 6 us, 1000 requests (3.8 MB in and out) 10 us.
 #include "ctmi_device.h"
 #include "ctmi_host.h"
 
@@ -191,12 +191,15 @@ extern "C" int ctmi_kv_plan(const int32_t* seq_lens, const int32_t* new_tokens, 
   PlanArgs a{seq_lens, new_tokens, block_table, free_blocks, num_free, width, free_capacity, slot_count,
              (int32_t)requests, block_size, seq_lens_out, query_start, slots, table_out, free_out,
              num_free_out, status};
-  // eight outputs a thread: fewer workgroups repeat the scan less, more of them hide its
-  // latency no better
+  // An output is a chain of dependent loads, so a thread has one, if the grid allows (1000
+  // requests 7.9 us, with eight a thread 14.3).  Each workgroup repeats the scan: of many requests
+  // one workgroup per compute unit does (4096 requests, 64 blocks each: 17 us, 41 with four times
+  // as many), of fewer up to four (1000 requests, 256 blocks each and 10^5 tokens: 10.0, one 13.3).
   const int64_t most = slot_count > requests * width ? slot_count : requests * width;
-  int64_t grid = cdiv(most > free_capacity ? most : free_capacity, (int64_t)kPlanThreads * 8);
+  int64_t grid = cdiv(most > free_capacity ? most : free_capacity, (int64_t)kPlanThreads);
+  const int64_t cap = requests > 1024 ? 256 : 1024;
   if (grid < 1) grid = 1;
-  if (grid > 1024) grid = 1024;
+  if (grid > cap) grid = cap;
   const size_t lds = (size_t)(requests + 1) * 3 * sizeof(int32_t);
   kv_plan_kernel<<<dim3((unsigned)grid), dim3(kPlanThreads), lds, (hipStream_t)stream>>>(a);
   return check_launch("kv_plan");
