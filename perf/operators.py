@@ -13,7 +13,6 @@ Data formats (the framework's):
   cache.value        [blocks, kv heads, head dim, block size]  8-bit codes
   cache.key_scale, cache.value_scale   fp32 [blocks, kv heads]
 """
-import functools
 import math
 import sys
 from pathlib import Path
@@ -29,9 +28,8 @@ CODE_MAX = {"fp8": 448.0, "int8": 127.5}  # half the range of the codes: max|x| 
 EPS = torch.finfo(torch.float32).eps  # smallest scale
 
 
-@functools.lru_cache(maxsize=None)
 def _package():
-    """the framework's entry points, imported where they are first called"""
+    """the framework's entry points, imported where they are called"""
     at = str(Path(__file__).resolve().parent.parent / "compressed-tensors_amd")
     if at not in sys.path:
         sys.path.insert(0, at)
