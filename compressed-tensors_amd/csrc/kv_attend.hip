@@ -9,7 +9,7 @@
 //
 //   S^T = K Q^T   4 key tiles x head_dim / 32 products 16x16x32; the codes become bf16 / f16
 //                 in registers (exact), the scales multiply the fp32 scores
-//   O^T = V^T P^T head_dim / 16 tiles x 2 products, P as bf16
+//   O^T = V^T P^T head_dim / 16 tiles x 2 products, P as one f16 or several bf16 numbers
 //
 // Both operands that come from memory are what the lanes already hold: a product's result has
 // its rows (keys) in lane group j = lane / 16 and its columns (query rows) in lane % 16, and
@@ -28,6 +28,8 @@
 // of up to 4096, 82 us, 5.5 TB/s (memory bounds it); 6 of up to 32768, 77 us, 5.0 TB/s, and 5 us
 // for the parts; 2 prompts of 2000 over 4000 keys 252 us, 0.71 PFLOP/s, vector units 55 % and
 // matrix cores 31 % busy: the softmax between the products bounds it.
+#include <type_traits>
+
 #include "kv_blocks.h"
 
 namespace ctmi {
@@ -36,6 +38,7 @@ namespace {
 constexpr int kAttendWaves = 4;
 constexpr int kStep = 64;  // keys per step of a wavefront
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLeastVs = 0x1p-90f, kMostVs = 0x1p90f;  // scales of values that are taken as they are
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -162,23 +165,37 @@ __device__ __forceinline__ Operand operand(const Operands& ready, int u) {
   return ready.half[u];
 }
 
+// What a weight of the softmax is held in for the second product: this many bf16 numbers that add
+// up to it (three are all 24 bits of fp32, two 16 of them), or one f16 number (11 bits).
+enum class Weights { kHalf = 1, kPair = 2, kTriple = 3 };
+
 // The rows of a wavefront and what they have gathered: RT tiles of 16, row `first` + 16 t + c
 // in lanes with lane % 16 == c.  UNIFORM: a step lies in one block, so its scales are one
 // number, and `sum` is the row's in all its lanes; otherwise each lane group has a part of it.
-template <typename T, bool FP8, int D, int RT, bool SPLIT, bool UNIFORM>
+//
+// `top` is the largest of score + log2(scale of the values), by which weight times scale is taken
+// from one exponential, as 2^7 at the top: what f16 loses at its lower end is then 2^-32 of the
+// largest product a key has, whatever the scales are.  `sum` has the weights alone, in the same
+// unit: with scales of 2^-90 at least it stays below 2^127.
+template <typename T, bool FP8, int D, int RT, Weights W, bool UNIFORM>
 struct AttendRows {
   static constexpr int CH = D / 64;  // 16-byte pieces of a key per lane
   static constexpr int DT = D / 16;  // tiles of the output's dimensions
+  static constexpr bool HALF = W == Weights::kHalf;
+  static constexpr int PARTS = (int)W;  // operands a weight takes
+  using V = std::conditional_t<HALF, F16, BF16>;
 
   Operand q[RT][CH][2];  // dimensions ch * 64 + j * 16 + half * 8 + 0 ... 7
   f32x4 o[RT][DT];       // dimension d * 16 + j * 4 + i
   float top[RT], sum[RT];
+  float most_vs;                           // the largest scale of values so far
   int ends[RT], seen_by_all, seen_by_any;  // keys seen: by each row, by the first and the last
 
   __device__ __forceinline__ void begin(const AttendArgs& a, const Request& rq, int first, int rows, int kv, int share) {
     const int c = lane_id() & 15, j = lane_id() >> 4;
     seen_by_any = first < rows ? last_key(rq, min(first + RT * 16, rows) - 1, share) : 0;
     seen_by_all = first < rows ? last_key(rq, first, share) : 0;
+    most_vs = 0.0f;
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
       const int row = first + t * 16 + c;
@@ -205,6 +222,25 @@ struct AttendRows {
       for (int ch = 0; ch < CH; ++ch)
 #pragma unroll
         for (int i = 0; i < 8; ++i) asm volatile("" : "+v"(q[t][ch][i / 4].w[i % 4]));
+  }
+
+  // the weights of two keys as operands
+  template <bool INFINITE>
+  static __device__ __forceinline__ void split(uint32_t* parts, float w0, float w1) {
+    if constexpr (HALF) {
+      typedef float f32x2 __attribute__((ext_vector_type(2)));
+      parts[0] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{w0, w1}), f16x2));
+    } else {
+#pragma unroll
+      for (int n = 0; n < PARTS; ++n) {
+        parts[n] = pack_bf16x2(w0, w1);
+        if (n + 1 < PARTS) {
+          // (nothing is left of an infinity)
+          w0 = INFINITE && fabsf(w0) == INFINITY ? 0.0f : w0 - u2f(parts[n] << 16);
+          w1 = INFINITE && fabsf(w1) == INFINITY ? 0.0f : w1 - u2f(parts[n] & 0xFFFF0000u);
+        }
+      }
+    }
   }
 
   // 64 keys from kb on.  key(t, ch): 16 bytes of this lane's row of key tile t; value(d): the
@@ -273,13 +309,18 @@ struct AttendRows {
 #pragma unroll
           for (int i = 0; i < 4; ++i) s[t][kt][i] = !valid || at16 + kt * 4 + i >= ends[t] ? -INFINITY : s[t][kt][i] * ks;
     }
-    Operand hi[RT][2], lo[RT][2];
-    auto weights = [](uint32_t& high, uint32_t& low, float w0, float w1) {
-      high = pack_bf16x2(w0, w1);
-      if constexpr (SPLIT) low = pack_bf16x2(w0 - u2f(high << 16), w1 - u2f(high & 0xFFFF0000u));
-    };
-    const bool plain = __all(vs > 0x1p-30f && vs < 0x1p30f);
-    const float log_vs = __builtin_amdgcn_logf(vs), by_vs = __builtin_amdgcn_rcpf(vs);
+    // plain: scales as they should be, and where the sum is of rounded numbers (below) none of
+    // them so small beside others that f16 would have lost what a weight adds to the sum
+    most_vs = fmaxf(most_vs, vs);
+    const bool plain = __all(vs >= kLeastVs && vs <= kMostVs && (!(HALF && UNIFORM) || vs * 256.0f >= most_vs));
+    float log_vs = __builtin_amdgcn_logf(vs), by_vs = __builtin_amdgcn_rcpf(vs), times = 1.0f;
+    if (!plain) {  // vs = 2^log_vs times
+      const float size = fabsf(vs);
+      const bool ordinary = size >= kLeastVs && size <= kMostVs;
+      log_vs = ordinary ? __builtin_amdgcn_logf(size) : size > kMostVs ? 90.0f : -90.0f;
+      times = ordinary ? copysignf(1.0f, vs) : vs * (size > kMostVs ? kLeastVs : kMostVs);
+    }
+    Operand w[RT][2][PARTS];
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
       float m = s[t][0][0];
@@ -287,10 +328,10 @@ struct AttendRows {
       for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
         for (int i = 0; i < 4; ++i) m = fmaxf(m, s[t][kt][i]);
-      m *= unit;
-      // weights may exceed 1 by 2^8 before the sums are brought to a new maximum: fp32 and
-      // bf16 keep their relative precision there, and the lanes of a row need not be asked
-      // for their maximum in most steps
+      m = fmaf(m, unit, log_vs);
+      // weights may exceed the top's by 2^8 before the sums are brought to a new one: the operands
+      // keep their precision there, and the lanes of a row need not be asked for their maximum in
+      // most steps
       if (__any(m > top[t] + 8.0f)) {
         const float now = fmaxf(top[t], groups_max(m));
         const float shrink = top[t] == -INFINITY ? 0.0f : exp2_fast(top[t] - now);
@@ -299,11 +340,9 @@ struct AttendRows {
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[t][d] *= shrink;
       }
-      const float base = top[t] == -INFINITY ? 0.0f : top[t];
+      const float base = (top[t] == -INFINITY ? 0.0f : top[t]) - 7.0f, less = base - log_vs;
+      float part = 0.0f;
       if (plain) {
-        // weight times scale in one exponential; the sum of weights takes the scale out again
-        const float less = base - log_vs;
-        float part = 0.0f;
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -311,32 +350,40 @@ struct AttendRows {
             const float w0 = exp2_fast(fmaf(s[t][u * 2 + e / 2][(e % 2) * 2], unit, -less));
             const float w1 = exp2_fast(fmaf(s[t][u * 2 + e / 2][(e % 2) * 2 + 1], unit, -less));
             if constexpr (!UNIFORM) part += w0 + w1;
-            weights(hi[t][u].w[e], lo[t][u].w[e], w0, w1);
+            uint32_t parts[PARTS];
+            split<false>(parts, w0, w1);
+#pragma unroll
+            for (int n = 0; n < PARTS; ++n) w[t][u][n].w[e] = parts[n];
           }
         if constexpr (UNIFORM) {
           // all weights carry the same scale: their sum is two products with ones
-          const Operand ones = {{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u}};
+          constexpr uint32_t one = HALF ? 0x3C003C00u : 0x3F803F80u;
+          const Operand ones = {{one, one, one, one}};
           f32x4 all = {0, 0, 0, 0};
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            all = product<BF16>(ones, hi[t][u], all);
-            if constexpr (SPLIT) all = product<BF16>(ones, lo[t][u], all);
-          }
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int n = 0; n < PARTS; ++n) all = product<V>(ones, w[t][u][n], all);
           part = all[0];
         }
         sum[t] = fmaf(part, by_vs, sum[t]);
       } else {
-        // the scale of a block that a row sees nothing of does not touch it, whatever it is
-        const float by = whole || (valid && at16 < ends[t]) ? vs : 0.0f;
-        float part = 0.0f;
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float p0 = exp2_fast(fmaf(s[t][u * 2 + e / 2][(e % 2) * 2], unit, -base));
-            const float p1 = exp2_fast(fmaf(s[t][u * 2 + e / 2][(e % 2) * 2 + 1], unit, -base));
-            part += p0 + p1;
-            weights(hi[t][u].w[e], lo[t][u].w[e], p0 * by, p1 * by);
+            float weight[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const float score = s[t][u * 2 + e / 2][(e % 2) * 2 + i];
+              part += exp2_fast(fmaf(score, unit, -base));
+              // a key that a row does not see does not touch it, whatever the scale of its block
+              weight[i] = score == -INFINITY ? 0.0f : exp2_fast(fmaf(score, unit, -less)) * times;
+            }
+            uint32_t parts[PARTS];
+            split<true>(parts, weight[0], weight[1]);
+#pragma unroll
+            for (int n = 0; n < PARTS; ++n) w[t][u][n].w[e] = parts[n];
           }
         sum[t] += UNIFORM ? groups_sum(part) : part;
       }
@@ -344,27 +391,26 @@ struct AttendRows {
     // (two loops: a branch for each d would leave each load of a value alone with its wait)
     __builtin_amdgcn_s_setprio(1);
     if constexpr (FP8) {
-      if (whole) gather(hi, lo, value);
-      else gather(hi, lo, [&](int d) { return clean(value(d), true); });
+      if (whole) gather(w, value);
+      else gather(w, [&](int d) { return clean(value(d), true); });
     } else {
-      gather(hi, lo, value);
+      gather(w, value);
     }
     __builtin_amdgcn_s_setprio(0);
   }
 
   template <typename Value>
-  __device__ __forceinline__ void gather(const Operand (*hi)[2], const Operand (*lo)[2], Value value) {
+  __device__ __forceinline__ void gather(const Operand (*w)[2][PARTS], Value value) {
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
-      const auto w = value(d);
+      const auto codes = value(d);
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const Operand v = operand<BF16, FP8>(w, u);
+        const Operand v = operand<V, FP8>(codes, u);
 #pragma unroll
-        for (int t = 0; t < RT; ++t) {
-          o[t][d] = product<BF16>(v, hi[t][u], o[t][d]);
-          if constexpr (SPLIT) o[t][d] = product<BF16>(v, lo[t][u], o[t][d]);
-        }
+        for (int t = 0; t < RT; ++t)
+#pragma unroll
+          for (int n = 0; n < PARTS; ++n) o[t][d] = product<V>(v, w[t][u][n], o[t][d]);
       }
     }
   }
@@ -434,7 +480,7 @@ __device__ __forceinline__ int64_t cell_of(const AttendArgs& a, int block, int k
 // from memory into the registers they are multiplied from
 template <typename T, bool FP8, int D, int RT>
 __global__ __launch_bounds__(kAttendWaves* kWave, D == 256 || RT == 2 ? 1 : 2) void kv_attend_split_kernel(AttendArgs a) {
-  using Rows = AttendRows<T, FP8, D, RT, true, false>;
+  using Rows = AttendRows<T, FP8, D, RT, Weights::kTriple, false>;
   constexpr int ROWS = RT * 16, CH = Rows::CH, DT = Rows::DT;
   const int lane = lane_id(), wave = threadIdx.x / kWave, c = lane & 15, j = lane >> 4;
   const int share = a.q_heads / a.kv_heads;
@@ -570,9 +616,9 @@ __global__ __launch_bounds__(kAttendWaves* kWave, D == 256 || RT == 2 ? 1 : 2) v
 //
 // WIDE: blocks are whole steps of 64 keys, so a step lies in one of them: its number, its
 // addresses and scales are the wavefront's and cost no vector instruction.
-template <typename T, bool FP8, int D, int RT, bool SPLIT, bool WIDE>
+template <typename T, bool FP8, int D, int RT, Weights W, bool WIDE>
 __global__ __launch_bounds__(kAttendWaves* kWave, D == 256 ? 1 : 2) void kv_attend_rows_kernel(AttendArgs a) {
-  using Rows = AttendRows<T, FP8, D, RT, SPLIT, WIDE>;
+  using Rows = AttendRows<T, FP8, D, RT, W, WIDE>;
   constexpr int ROWS = kAttendWaves * RT * 16, PIECES = D / 64;  // 16-byte pieces a thread loads of either
   constexpr int KP = D / 16;                                     // pieces of a key
   constexpr int KEYS = kAttendWaves * kWave / KP;                // keys per round of loads
@@ -674,7 +720,7 @@ __global__ __launch_bounds__(kAttendWaves* kWave, D == 256 ? 1 : 2) void kv_atte
           for (int u = 0; u < 2; ++u) {
             using Bits = Vec<uint32_t, 4>;
             keys[half][key_place(key, my_piece * 2 + u)] = __builtin_bit_cast(Bits, operand<T, FP8>(kr[p], u));
-            values[half][value_place(d, my_group * 2 + u)] = __builtin_bit_cast(Bits, operand<BF16, FP8>(vr[p], u));
+            values[half][value_place(d, my_group * 2 + u)] = __builtin_bit_cast(Bits, operand<typename Rows::V, FP8>(vr[p], u));
           }
         }
       }
@@ -790,6 +836,13 @@ __global__ __launch_bounds__(kAttendWaves* kWave) void kv_attend_join_kernel(Att
   }
 }
 
+// Weights where rows are many and products the bound: bf16 outputs take one f16 number (2^-11 of
+// the weight, a quarter of half an output's step, at the price of one bf16 number; two numbers would
+// take 295 for 246 us at 2 x 2000 queries over 4000 keys), f16 outputs two bf16 numbers (2^-16).
+// Where rows are few memory is the bound and weights keep all their bits.
+template <typename T>
+constexpr Weights kRows = T::id == CTMI_F16 ? Weights::kPair : Weights::kHalf;
+
 // the launch: which kernel, how many tiles of rows and chunks of keys a request gets
 struct Launch {
   bool split_keys;
@@ -895,15 +948,13 @@ extern "C" int ctmi_kv_attend(const void* q, int32_t dtype, int64_t q_token_stri
   const hipStream_t s = (hipStream_t)stream;
   const dim3 blocks_of((unsigned)grid), threads(kAttendWaves * kWave);
   const bool fp8 = blocks->code_dtype == CTMI_F8E4M3;
-  // bf16 outputs of long prompts take the weights as one bf16 number (2^-8, half a step of the
-  // output's type); elsewhere they are two, which costs nothing while memory is the bound
 #define BY_TILE(T, F, D)                                                                                           \
   do {                                                                                                             \
     constexpr int RT2 = D == 256 ? 1 : 2;                                                                          \
     if (!l.split_keys && a.block_size % kStep == 0)                                                                \
-      kv_attend_rows_kernel<T, F, D, RT2, T::id == CTMI_F16, true><<<blocks_of, threads, 0, s>>>(a);               \
+      kv_attend_rows_kernel<T, F, D, RT2, kRows<T>, true><<<blocks_of, threads, 0, s>>>(a);               \
     else if (!l.split_keys)                                                                                        \
-      kv_attend_rows_kernel<T, F, D, RT2, T::id == CTMI_F16, false><<<blocks_of, threads, 0, s>>>(a);              \
+      kv_attend_rows_kernel<T, F, D, RT2, kRows<T>, false><<<blocks_of, threads, 0, s>>>(a);              \
     else if (RT2 == 1 || l.row_tiles == 1) kv_attend_split_kernel<T, F, D, 1><<<blocks_of, threads, 0, s>>>(a);    \
     else kv_attend_split_kernel<T, F, D, RT2><<<blocks_of, threads, 0, s>>>(a);                                    \
     if (cells) kv_attend_join_kernel<T, D><<<dim3((unsigned)join), threads, 0, s>>>(a, l.tile_rows, (int)max_query); \
