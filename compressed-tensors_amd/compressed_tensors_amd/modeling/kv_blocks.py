@@ -130,12 +130,13 @@ def append_kv_blocks(key: Tensor, value: Tensor, blocks: KVBlocks, slots: Tensor
 
     `slots[t]` is block * block_size + position of token t; one outside the pool (-1) skips the
     token.  Tokens of one block stand next to each other in rising order and a slot is named
-    once, as `plan_kv_blocks` gives them.
+    once, as `plan_kv_blocks` gives them.  Where slots are left out, or tokens skipped, inside a
+    block, its runs of consecutive slots are written one after the other, as by calls of their own.
 
     dynamic: the scale of a block and head is the largest new |x| over half the range of the
     codes (448 or 127.5), never below fp32's eps, and never falls while the block fills; where
     it grows, the block's older codes are rewritten to it.  A block whose first position is
-    among the new tokens starts afresh.  Otherwise the scales are the caller's and x / scale
+    a new token's starts afresh.  Otherwise the scales are the caller's and x / scale
     saturates.  Forward only."""
     c = _describe(blocks)
     if key.ndim != 3 or value.shape != key.shape or key.shape[1] != c.kv_heads or key.shape[2] != c.head_dim:

@@ -94,13 +94,180 @@ __device__ __forceinline__ uint32_t rescale4(uint32_t w, float ratio, int count)
   return (o & mask) | (w & ~mask);
 }
 
+// The run of tokens t ... t + n - 1, positions at ... of a block, whose scale is `was`; returns what
+// it is afterwards.  peaks: LDS that no wavefront still reads for the run before.
 template <typename T, bool FP8, int D, int side>
-__device__ __forceinline__ void append_window(const AppendArgs& a) {
+__device__ __forceinline__ float append_run(const AppendArgs& a, int64_t t, int n, int at, int head, int stride, float was,
+                                            uint8_t* codes, float* scale, uint32_t* peaks) {
   constexpr int CH = D / 4;  // pieces of 4 dimensions
   // What a thread loads for the maximum and keeps for the codes: 8 pieces, those of 8 tokens
   // (keys) or of the 4 tokens of 2 words (values).  That is 64 tokens of 128 dimensions; the
   // rest of a longer run is read twice.
   constexpr int KEEP = 8;
+  const int bs = a.block_size, lane = lane_id();
+  const uint16_t* x = a.x[side] + t * a.token_stride[side] + head * a.head_stride[side];
+  // keys: piece i is 4 dimensions of token i / CH.  Values: item i is 4 dimensions of the 4
+  // tokens of a word, of which those outside the run are read as its nearest; words of a row
+  // of the block are lanes next to each other
+  const int word0 = at / 4, words = (at + n + 3) / 4 - word0, items = side == 0 ? n * CH : words * CH;
+  const uint32_t magic = 0xFFFFFFFFu / (uint32_t)words + 1;  // i / words for the i there are (words > 1)
+  auto row_of = [&](int i) { return words == 1 ? i : (int)__umulhi((uint32_t)i, magic); };
+  auto key_piece = [&](int i) { return ldg<uint16_t, 4>(x + (uint32_t)((i / CH) * stride + (i % CH) * 4)); };
+  auto first_token = [&](int i) { return (word0 + i - row_of(i) * words) * 4 - at; };
+  auto value_piece = [&](int i, int e) {
+    return ldg<uint16_t, 4>(x + (uint32_t)(min(max(first_token(i) + e, 0), n - 1) * stride + row_of(i) * 4));
+  };
+  // magnitudes order like the unsigned integers of their bits, infinities and NaNs above all
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  u16x2 most = {0, 0};
+  auto look = [&](const Vec<uint16_t, 4>& v) {
+    const Vec<uint32_t, 2> w = __builtin_bit_cast(Vec<uint32_t, 2>, v);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, w.v[e] & 0x7FFF7FFFu));
+  };
+  Vec<uint16_t, 4> kept[KEEP];
+#pragma unroll
+  for (int p = 0; p < KEEP; ++p) {
+    // behind the last one the last: loads that stand in no branch
+    const int i = min((int)threadIdx.x + (side == 0 ? p : p / 4) * kAppendThreads, items - 1);
+    kept[p] = side == 0 ? key_piece(i) : value_piece(i, p % 4);
+  }
+#pragma unroll
+  for (int p = 0; p < KEEP; ++p) look(kept[p]);
+  if (side == 0) {
+#pragma unroll 1
+    for (int i = threadIdx.x + KEEP * kAppendThreads; i < items; i += kAppendThreads) look(key_piece(i));
+  } else {
+#pragma unroll 1
+    for (int i = threadIdx.x + KEEP / 4 * kAppendThreads; i < items; i += kAppendThreads)
+      for (int e = 0; e < 4; ++e) look(value_piece(i, e));
+  }
+  // (the other half of peaks may still be read for the run before)
+  uint32_t high = most[0] > most[1] ? most[0] : most[1];
+#pragma unroll
+  for (int m = 1; m < kWave; m *= 2) high = max(high, (uint32_t)wave_shfl_xor((int)high, m));
+  if (lane == 0) peaks[threadIdx.x / kWave] = high;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kAppendThreads / kWave; ++w) high = max(high, peaks[w]);
+  constexpr uint32_t kInfinity = T::id == CTMI_BF16 ? 0x7F80u : 0x7C00u;
+  const bool strange = high >= kInfinity;
+  if (strange) {  // the largest that is finite, element by element
+    high = 0;
+#pragma unroll 1
+    for (int i = threadIdx.x; i < n * D; i += kAppendThreads) {
+      const uint32_t m = x[(i / D) * stride + i % D] & 0x7FFFu;
+      high = m < kInfinity ? max(high, m) : high;
+    }
+#pragma unroll
+    for (int m = 1; m < kWave; m *= 2) high = max(high, (uint32_t)wave_shfl_xor((int)high, m));
+    __syncthreads();
+    if (lane == 0) peaks[threadIdx.x / kWave] = high;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kAppendThreads / kWave; ++w) high = max(high, peaks[w]);
+  }
+  const float peak = T::to_f32((uint16_t)high);
+
+  float now = was;
+  if (a.dynamic) {
+    const float fits = fmaxf(peak / (FP8 ? 448.0f : 127.5f), kScaleFloor);
+    now = at == 0 ? fits : fmaxf(was, fits);
+    if (at > 0 && now != was) {
+      const float ratio = was / now;
+      if (side == 0) {
+        uint32_t* w = (uint32_t*)codes;
+#pragma unroll 1
+        for (int i = threadIdx.x; i < at * (D / 4); i += kAppendThreads) w[i] = rescale4<FP8>(w[i], ratio, 4);
+      } else {
+        const int old = (at + 3) / 4;
+#pragma unroll 1
+        for (int i = threadIdx.x; i < old * D; i += kAppendThreads) {
+          uint32_t* w = (uint32_t*)(codes + (i / old) * bs) + i % old;
+          *w = rescale4<FP8>(*w, ratio, at - (i % old) * 4);
+        }
+      }
+      __syncthreads();  // words that old and new codes share are rewritten before the new ones come
+    }
+    if (threadIdx.x == 0) *scale = now;
+  }
+
+  if (strange || !(now > 0x1p-100f && now < 0x1p100f && peak <= now * 65536.0f)) {
+#pragma unroll 1
+    for (int i = threadIdx.x; i < n * D; i += kAppendThreads) {
+      const int token = i / D, d = i % D;
+      codes[side == 0 ? (at + token) * D + d : d * bs + at + token] = encode<FP8>(T::to_f32(x[token * stride + d]) / now);
+    }
+    return now;
+  }
+  const Divisor by{now, 1.0f / now};
+  if (side == 0) {
+#pragma unroll
+    for (int p = 0; p < KEEP; ++p) {
+      const int i = threadIdx.x + p * kAppendThreads;
+      if (i < items) *(uint32_t*)(codes + at * D + i * 4) = encode4<T, FP8>(kept[p], by);
+    }
+#pragma unroll 1
+    for (int i = threadIdx.x + KEEP * kAppendThreads; i < items; i += kAppendThreads)
+      *(uint32_t*)(codes + at * D + i * 4) = encode4<T, FP8>(key_piece(i), by);
+  } else {
+#pragma unroll 1
+    for (int i = threadIdx.x, turn = 0; i < items; i += kAppendThreads, ++turn) {
+      uint32_t o[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        o[e] = encode4<T, FP8>(turn == 0 ? kept[e] : turn == 1 ? kept[4 + e] : value_piece(i, e), by);
+      const int first = first_token(i);
+      uint8_t* row = codes + (row_of(i) * 4) * bs + at + first;
+      if (first >= 0 && first + 4 <= n) {
+        // 4 tokens x 4 dimensions of bytes, transposed
+        const uint32_t a01 = __builtin_amdgcn_perm(o[1], o[0], 0x05010400u), b01 = __builtin_amdgcn_perm(o[1], o[0], 0x07030602u);
+        const uint32_t a23 = __builtin_amdgcn_perm(o[3], o[2], 0x05010400u), b23 = __builtin_amdgcn_perm(o[3], o[2], 0x07030602u);
+        *(uint32_t*)row = __builtin_amdgcn_perm(a23, a01, 0x05040100u);
+        *(uint32_t*)(row + bs) = __builtin_amdgcn_perm(a23, a01, 0x07060302u);
+        *(uint32_t*)(row + 2 * bs) = __builtin_amdgcn_perm(b23, b01, 0x05040100u);
+        *(uint32_t*)(row + 3 * bs) = __builtin_amdgcn_perm(b23, b01, 0x07060302u);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (first + e >= 0 && first + e < n) {
+#pragma unroll
+            for (int d = 0; d < 4; ++d) row[d * bs + e] = (uint8_t)(o[e] >> (8 * d));
+          }
+      }
+    }
+  }
+  return now;
+}
+
+constexpr uint32_t kNoSlot = 0x80000000u;
+
+// the slot of the first token from `from` on that has one, and which token that is; 512 at a time,
+// as the rest of a padded batch has none
+__device__ __forceinline__ uint32_t next_slot(const AppendArgs& a, int64_t from, int64_t* token) {
+  constexpr int FAR = 8;
+  uint32_t slot = kNoSlot;
+  for (; from < a.tokens && slot == kNoSlot; from += FAR * kWave) {
+    int64_t there[FAR];
+#pragma unroll
+    for (int f = 0; f < FAR; ++f) {
+      const int64_t at = from + f * kWave + lane_id();
+      there[f] = at < a.tokens ? a.slots[at] : -1;
+    }
+#pragma unroll
+    for (int f = 0; f < FAR; ++f) {
+      const uint64_t any = __ballot((uint64_t)there[f] < (uint64_t)a.pool);
+      if (any && slot == kNoSlot) {
+        slot = __builtin_amdgcn_readlane((uint32_t)there[f], __builtin_ctzll(any));
+        *token = from + f * kWave + __builtin_ctzll(any);
+      }
+    }
+  }
+  return slot;
+}
+
+template <typename T, bool FP8, int D, int side>
+__device__ __forceinline__ void append_window(const AppendArgs& a) {
   const int head = blockIdx.y, bs = a.block_size, lane = lane_id();
   const int stride = (int)a.token_stride[side];
   const int64_t t0 = (int64_t)blockIdx.x * a.window;
@@ -111,23 +278,55 @@ __device__ __forceinline__ void append_window(const AppendArgs& a) {
   const int64_t mine = t0 - 1 + lane;
   const int64_t wide = mine >= 0 && mine < a.tokens ? a.slots[mine] : -1;
   const bool valid = (uint64_t)wide < (uint64_t)a.pool;
-  const uint32_t slot_here = valid ? (uint32_t)wide : 0x80000000u;
+  const uint32_t slot_here = valid ? (uint32_t)wide : kNoSlot;
   const uint32_t slot_before = __shfl_up(slot_here, 1, kWave);
   const uint32_t block_here = a.magic ? __umulhi(slot_here >> 4, a.magic) : slot_here >> 4;
   const int at_here = (int)(slot_here - block_here * (uint32_t)bs);
-  const bool goes_on = valid && at_here > 0 && lane > 0 && slot_before == slot_here - 1;
-  const uint64_t follows = __ballot(goes_on);
-  int parity = 0;
-  for (uint64_t left = __ballot(valid && !goes_on && lane > 0 && lane <= a.window); left; left &= left - 1, parity ^= 1) {
-    const int lead = __builtin_ctzll(left);
-    const int64_t t = t0 - 1 + lead, block = (int64_t)__shfl(block_here, lead, kWave);
-    const int at = __shfl(at_here, lead, kWave);
-    uint8_t* codes = a.codes[side] + (block * a.kv_heads + head) * (int64_t)bs * D;
-    float* scale = a.scales[side] + block * a.kv_heads + head;
-    const float was = *scale;
-    const uint64_t behind = lead == 63 ? 0 : ~(follows >> (lead + 1));  // 0 bits: tokens of the run
-    int n = 1 + (lead == 63 ? 0 : __builtin_ctzll(behind | 1ull << (63 - lead)));
-    if (lead + n == kWave) {  // it may go on behind what was looked at
+  // the token before lies before it in the same block: it goes on with that one's run, or has a
+  // later one of the block
+  const bool later = valid && slot_before < slot_here && slot_before >= slot_here - (uint32_t)at_here && lane > 0;
+  const bool goes_on = later && slot_before == slot_here - 1;
+  const uint64_t follows = __ballot(goes_on), valids = __ballot(valid);
+  // behind whose predecessor the block may have another run
+  const uint64_t chained = __ballot((later && !goes_on) || (!valid && slot_before != kNoSlot && mine < a.tokens));
+  auto same_block = [&](uint32_t slot, uint32_t before) {
+    const uint32_t block = a.magic ? __umulhi(slot >> 4, a.magic) : slot >> 4;
+    return before < slot && before >= block * (uint32_t)bs;
+  };
+  bool begins = valid && !later && lane > 0 && lane <= a.window;
+  // (behind tokens that are skipped it lies further back)
+  if (__builtin_expect(__any(begins && slot_before == kNoSlot), 0)) {
+    const uint64_t before_me = valids & ((1ull << lane) - 1);
+    const uint32_t last_before = __shfl(slot_here, before_me ? 63 - __builtin_clzll(before_me) : 0, kWave);
+    if (before_me && same_block(slot_here, last_before)) begins = false;
+    const int first_valid = __builtin_ctzll(valids);
+    for (int64_t base = t0 - 2; first_valid > 0 && base >= 0; base -= kWave) {
+      const int64_t there = base - lane >= 0 ? a.slots[base - lane] : -1;
+      const uint64_t any = __ballot((uint64_t)there < (uint64_t)a.pool);
+      if (any) {
+        const uint32_t slot = __builtin_amdgcn_readlane((uint32_t)there, __builtin_ctzll(any));
+        if (lane == first_valid && same_block(slot_here, slot)) begins = false;
+        break;
+      }
+    }
+  }
+  uint64_t left = __ballot(begins);
+  int lead = 0, at = 0;  // the run's first token (one behind what was looked at: kWave), its position
+  int64_t t = 0, block = 0;
+  float was = 0.0f;
+  bool same = false;  // the block is that of the run before
+  for (int parity = 0; same || left; parity ^= 1) {
+    if (!same) {
+      lead = __builtin_ctzll(left);
+      left &= left - 1;
+      t = t0 - 1 + lead;
+      block = (int64_t)__builtin_amdgcn_readlane(block_here, lead);
+      at = __builtin_amdgcn_readlane(at_here, lead);
+      was = a.scales[side][block * a.kv_heads + head];
+    }
+    const uint64_t behind = lead >= 63 ? 0 : ~(follows >> (lead + 1));  // 0 bits: tokens of the run
+    int n = 1 + (lead >= 63 ? 0 : __builtin_ctzll(behind | 1ull << (63 - lead)));
+    if (lead + n >= kWave) {  // it may go on behind what was looked at
       const int64_t slot = block * bs + at;
       for (const int most = bs - at; n < most;) {
         const int i = n + lane;
@@ -139,137 +338,26 @@ __device__ __forceinline__ void append_window(const AppendArgs& a) {
         n += kWave;
       }
     }
+    const int64_t cell = block * a.kv_heads + head;
+    was = append_run<T, FP8, D, side>(a, t, n, at, head, stride, was, a.codes[side] + cell * bs * D, a.scales[side] + cell, peaks[parity]);
 
-    const uint16_t* x = a.x[side] + t * a.token_stride[side] + head * a.head_stride[side];
-    // keys: piece i is 4 dimensions of token i / CH.  Values: item i is 4 dimensions of the 4
-    // tokens of a word, of which those outside the run are read as its nearest; words of a row
-    // of the block are lanes next to each other
-    const int word0 = at / 4, words = (at + n + 3) / 4 - word0, items = side == 0 ? n * CH : words * CH;
-    const uint32_t magic = 0xFFFFFFFFu / (uint32_t)words + 1;  // i / words for the i there are (words > 1)
-    auto row_of = [&](int i) { return words == 1 ? i : (int)__umulhi((uint32_t)i, magic); };
-    auto key_piece = [&](int i) { return ldg<uint16_t, 4>(x + (uint32_t)((i / CH) * stride + (i % CH) * 4)); };
-    auto first_token = [&](int i) { return (word0 + i - row_of(i) * words) * 4 - at; };
-    auto value_piece = [&](int i, int e) {
-      return ldg<uint16_t, 4>(x + (uint32_t)(min(max(first_token(i) + e, 0), n - 1) * stride + row_of(i) * 4));
-    };
-    // magnitudes order like the unsigned integers of their bits, infinities and NaNs above all
-    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
-    u16x2 most = {0, 0};
-    auto look = [&](const Vec<uint16_t, 4>& v) {
-      const Vec<uint32_t, 2> w = __builtin_bit_cast(Vec<uint32_t, 2>, v);
-#pragma unroll
-      for (int e = 0; e < 2; ++e) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, w.v[e] & 0x7FFF7FFFu));
-    };
-    Vec<uint16_t, 4> kept[KEEP];
-#pragma unroll
-    for (int p = 0; p < KEEP; ++p) {
-      // behind the last one the last: loads that stand in no branch
-      const int i = min((int)threadIdx.x + (side == 0 ? p : p / 4) * kAppendThreads, items - 1);
-      kept[p] = side == 0 ? key_piece(i) : value_piece(i, p % 4);
-    }
-#pragma unroll
-    for (int p = 0; p < KEEP; ++p) look(kept[p]);
-    if (side == 0) {
-#pragma unroll 1
-      for (int i = threadIdx.x + KEEP * kAppendThreads; i < items; i += kAppendThreads) look(key_piece(i));
-    } else {
-#pragma unroll 1
-      for (int i = threadIdx.x + KEEP / 4 * kAppendThreads; i < items; i += kAppendThreads)
-        for (int e = 0; e < 4; ++e) look(value_piece(i, e));
-    }
-    // (the other half of peaks may still be read for the run before)
-    uint32_t high = most[0] > most[1] ? most[0] : most[1];
-#pragma unroll
-    for (int m = 1; m < kWave; m *= 2) high = max(high, (uint32_t)wave_shfl_xor((int)high, m));
-    if (lane == 0) peaks[parity][threadIdx.x / kWave] = high;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kAppendThreads / kWave; ++w) high = max(high, peaks[parity][w]);
-    constexpr uint32_t kInfinity = T::id == CTMI_BF16 ? 0x7F80u : 0x7C00u;
-    const bool strange = high >= kInfinity;
-    if (strange) {  // the largest that is finite, element by element
-      high = 0;
-#pragma unroll 1
-      for (int i = threadIdx.x; i < n * D; i += kAppendThreads) {
-        const uint32_t m = x[(i / D) * stride + i % D] & 0x7FFFu;
-        high = m < kInfinity ? max(high, m) : high;
+    // the block's next run: of the nearest token behind that has a slot
+    same = false;
+    if (at + n < bs && (lead + n >= kWave || (chained >> (lead + n) & 1))) {
+      const uint64_t ahead = lead + n < kWave ? valids >> (lead + n) : 0;
+      uint32_t next;
+      if (ahead) {
+        lead += n + __builtin_ctzll(ahead);
+        t = t0 - 1 + lead;
+        next = __builtin_amdgcn_readlane(slot_here, lead);
+      } else {
+        next = next_slot(a, t + n > t0 - 1 + kWave ? t + n : t0 - 1 + kWave, &t);
+        lead = kWave;
       }
-#pragma unroll
-      for (int m = 1; m < kWave; m *= 2) high = max(high, (uint32_t)wave_shfl_xor((int)high, m));
-      __syncthreads();
-      if (lane == 0) peaks[parity][threadIdx.x / kWave] = high;
-      __syncthreads();
-#pragma unroll
-      for (int w = 0; w < kAppendThreads / kWave; ++w) high = max(high, peaks[parity][w]);
-    }
-    const float peak = T::to_f32((uint16_t)high);
-
-    float now = was;
-    if (a.dynamic) {
-      const float fits = fmaxf(peak / (FP8 ? 448.0f : 127.5f), kScaleFloor);
-      now = at == 0 ? fits : fmaxf(was, fits);
-      if (at > 0 && now != was) {
-        const float ratio = was / now;
-        if (side == 0) {
-          uint32_t* w = (uint32_t*)codes;
-#pragma unroll 1
-          for (int i = threadIdx.x; i < at * (D / 4); i += kAppendThreads) w[i] = rescale4<FP8>(w[i], ratio, 4);
-        } else {
-          const int old = (at + 3) / 4;
-#pragma unroll 1
-          for (int i = threadIdx.x; i < old * D; i += kAppendThreads) {
-            uint32_t* w = (uint32_t*)(codes + (i / old) * bs) + i % old;
-            *w = rescale4<FP8>(*w, ratio, at - (i % old) * 4);
-          }
-        }
-        __syncthreads();  // words that old and new codes share are rewritten before the new ones come
-      }
-      if (threadIdx.x == 0) *scale = now;
-    }
-
-    if (strange || !(now > 0x1p-100f && now < 0x1p100f && peak <= now * 65536.0f)) {
-#pragma unroll 1
-      for (int i = threadIdx.x; i < n * D; i += kAppendThreads) {
-        const int token = i / D, d = i % D;
-        codes[side == 0 ? (at + token) * D + d : d * bs + at + token] = encode<FP8>(T::to_f32(x[token * stride + d]) / now);
-      }
-      continue;
-    }
-    const Divisor by{now, 1.0f / now};
-    if (side == 0) {
-#pragma unroll
-      for (int p = 0; p < KEEP; ++p) {
-        const int i = threadIdx.x + p * kAppendThreads;
-        if (i < items) *(uint32_t*)(codes + at * D + i * 4) = encode4<T, FP8>(kept[p], by);
-      }
-#pragma unroll 1
-      for (int i = threadIdx.x + KEEP * kAppendThreads; i < items; i += kAppendThreads)
-        *(uint32_t*)(codes + at * D + i * 4) = encode4<T, FP8>(key_piece(i), by);
-    } else {
-#pragma unroll 1
-      for (int i = threadIdx.x, turn = 0; i < items; i += kAppendThreads, ++turn) {
-        uint32_t o[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          o[e] = encode4<T, FP8>(turn == 0 ? kept[e] : turn == 1 ? kept[4 + e] : value_piece(i, e), by);
-        const int first = first_token(i);
-        uint8_t* row = codes + (row_of(i) * 4) * bs + at + first;
-        if (first >= 0 && first + 4 <= n) {
-          // 4 tokens x 4 dimensions of bytes, transposed
-          const uint32_t a01 = __builtin_amdgcn_perm(o[1], o[0], 0x05010400u), b01 = __builtin_amdgcn_perm(o[1], o[0], 0x07030602u);
-          const uint32_t a23 = __builtin_amdgcn_perm(o[3], o[2], 0x05010400u), b23 = __builtin_amdgcn_perm(o[3], o[2], 0x07030602u);
-          *(uint32_t*)row = __builtin_amdgcn_perm(a23, a01, 0x05040100u);
-          *(uint32_t*)(row + bs) = __builtin_amdgcn_perm(a23, a01, 0x07060302u);
-          *(uint32_t*)(row + 2 * bs) = __builtin_amdgcn_perm(b23, b01, 0x05040100u);
-          *(uint32_t*)(row + 3 * bs) = __builtin_amdgcn_perm(b23, b01, 0x07060302u);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (first + e >= 0 && first + e < n) {
-#pragma unroll
-              for (int d = 0; d < 4; ++d) row[d * bs + e] = (uint8_t)(o[e] >> (8 * d));
-            }
-        }
+      if (next != kNoSlot && same_block(next, (uint32_t)(block * bs) + at + n - 1)) {
+        at = (int)(next - (uint32_t)(block * bs));
+        same = true;
+        __syncthreads();  // the run before has written its codes
       }
     }
   }

@@ -761,13 +761,15 @@ typedef struct ctmi_kv_blocks {
  * strides in elements (head_dim contiguous; multiples of 8, tokens below 2^22 apart; both
  * tensors 16-byte aligned), the pool of fewer than 2^31 slots.  slots: int64 [tokens],
  * block * block_size + position, tokens of one block next to each other in rising order (what
- * ctmi_kv_plan writes); a slot outside the pool (-1) skips its token.  A slot named twice in
- * one call is the caller's mistake: the block it names then holds either token's codes, under
- * either's scale.
- * dynamic != 0: with A = max|x| over the finite new values of a block and head, the scale
+ * ctmi_kv_plan writes); a slot outside the pool (-1) skips its token.  Consecutive slots of a
+ * block are a run; where slots are left out or tokens skipped inside a block, its runs are
+ * written one after the other, as calls of their own would.  A slot named twice in one call is
+ * the caller's mistake: the block it names then holds either token's codes, under either's scale.
+ * dynamic != 0: with A = max|x| over the finite new values of a run and head, the scale
  * becomes max(A / q, eps), or the maximum of that and the scale it had unless the block's
- * first position is among the new ones; q = 448 (e4m3) or 127.5 (int8), eps = 2^-23.  Codes
- * of the positions before the new ones become round(code * (old scale / new scale)).
+ * first position is the run's first; q = 448 (e4m3) or 127.5 (int8), eps = 2^-23.  Codes
+ * of the positions before the run become round(code * (old scale / new scale)); positions
+ * behind it hold nothing from then on.
  * dynamic == 0: the scales are the caller's and stay.  New codes are x / scale, clamped to
  * +-448 or [-128, 127] and rounded to nearest even; NaN becomes NaN (e4m3) or 0 (int8). */
 int ctmi_kv_append(const void* key, const void* value, int32_t dtype, int64_t key_token_stride,
