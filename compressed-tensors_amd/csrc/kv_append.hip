@@ -63,12 +63,13 @@ __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) 
   }
 }
 
-// x / s, correctly rounded, for finite x and s within 2^+-100; r = 1 / s
+// x / s, correctly rounded, for finite x and s within 2^+-100; r = 1 / s.  The remainders are taken
+// as q s - x: of x = -0 that is +0, and -0 less +0 r stays -0 (x - q s would make it +0).
 struct Divisor {
   float s, r;
   __device__ __forceinline__ float operator()(float x) const {
-    const float q = x * r, q1 = fmaf(fmaf(-q, s, x), r, q);
-    return fmaf(fmaf(-q1, s, x), r, q1);
+    const float q = x * r, q1 = fmaf(fmaf(q, s, -x), -r, q);
+    return fmaf(fmaf(q1, s, -x), -r, q1);
   }
 };
 
