@@ -424,6 +424,12 @@ SIGNATURES = {
          c_int64, c_int64, c_void_p, c_void_p, c_int64, c_float, c_int64, c_int64, c_void_p, c_int64,
          c_void_p],
     ),
+    "ctmi_kv_attend_padded": (
+        c_int32,
+        [c_void_p, c_int32, c_int64, c_int64, c_void_p, c_int64, c_int32, POINTER(KVBlocksC), c_void_p,
+         c_int64, c_int64, c_void_p, c_void_p, c_int64, c_float, c_int64, c_int64, c_void_p, c_int64,
+         c_void_p],
+    ),
     "ctmi_kv_plan": (
         c_int32,
         [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int32,

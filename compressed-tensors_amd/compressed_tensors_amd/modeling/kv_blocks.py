@@ -180,7 +180,8 @@ def attend_kv_blocks(query: Tensor, blocks: KVBlocks, block_table: Tensor, seq_l
 
     `max_query` and `max_seq`, the longest request's queries and keys, only choose the launch
     (defaults: all tokens, the table's width); any values give the right result.  Rows of
-    tokens outside every request (a padded batch) keep what `out` holds.  Forward only."""
+    tokens outside every request (a padded batch) keep what `out` holds; without `out` they are
+    zeros.  Forward only."""
     c = _describe(blocks)
     if query.ndim != 3 or query.shape[2] != c.head_dim or query.shape[1] < 1 or query.shape[1] % c.kv_heads:
         raise ValueError(f"expected queries [tokens, a multiple of {c.kv_heads}, {c.head_dim}], got {tuple(query.shape)}")
@@ -217,12 +218,17 @@ def attend_kv_blocks(query: Tensor, blocks: KVBlocks, block_table: Tensor, seq_l
     max_seq = max(1, longest if max_seq is None else min(max_seq, longest))
     scale = dim ** -0.5 if softmax_scale is None else float(softmax_scale)
     lib = _lib.load()
+    call = lib.ctmi_kv_attend
     if out is None:
+        if requests == 0:
+            return query.new_zeros((tokens, heads, dim))
         out = query.new_empty((tokens, heads, dim))
+        if query_start is not None:
+            call = lib.ctmi_kv_attend_padded
     tmp_bytes = lib.ctmi_kv_attend_tmp_bytes(tokens, requests, heads, c.kv_heads, dim, max_query, max_seq)
     tmp = torch.empty(tmp_bytes, dtype=torch.uint8, device=out.device) if tmp_bytes else None
     token_stride, head_stride, _ = query.stride()
-    _lib.check(lib.ctmi_kv_attend(
+    _lib.check(call(
         query.data_ptr(), _lib.dtype_code(query.dtype), token_stride, head_stride, out.data_ptr(), tokens, heads,
         ctypes.byref(c), block_table.data_ptr(), table_stride, width, lens.data_ptr(), _lib.ptr(query_start), requests,
         scale, max_query, max_seq, _lib.ptr(tmp), tmp_bytes, _lib.stream_of_index(index)))
@@ -235,8 +241,8 @@ class BlockKVCache:
     A serving step is `plan(new_tokens, total)`, then for each layer `update(layer, key,
     value)` and `attend(layer, query)`.  Everything stays on the GPU: nothing here waits for
     it except `check()`.  A step that does not fit changes nothing: `update` then writes
-    nothing and `attend` leaves its rows as they are.  `plan` replaces the cache's tensors; a
-    captured graph calls the functions on buffers of its own."""
+    nothing and `attend` gives zeros, or leaves `out` as it is.  `plan` replaces the cache's
+    tensors; a captured graph calls the functions on buffers of its own."""
 
     def __init__(self, layers: int, num_blocks: int, max_requests: int, max_blocks_per_request: int,
                  kv_heads: int, head_dim: int, block_size: int = 64,

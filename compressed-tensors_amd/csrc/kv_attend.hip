@@ -59,6 +59,7 @@ struct AttendArgs {
   int32_t tiles, chunks, chunk_keys;  // of the grid
   uint32_t sixteenths, magic;         // block_size / 16 and ceil(2^32 / that) (0: it is 1)
   float scale;                        // times log2(e)
+  int32_t clear;                      // rows of no request become zeros
 };
 
 struct Request {
@@ -476,6 +477,25 @@ __device__ __forceinline__ int64_t cell_of(const AttendArgs& a, int block, int k
   return (int64_t)(in_pool(a, block) ? block : 0) * a.kv_heads + kv;
 }
 
+// Rows before the first request's and behind the last one's, which become zeros if they are to, a
+// share by each workgroup when it is done.  Where they are is asked for when it begins: at the end
+// the answer would be waited for (0.5 us).
+struct Rest {
+  int before, behind;
+  __device__ __forceinline__ explicit Rest(const AttendArgs& a) : before(0), behind(a.tokens) {
+    if (a.clear) before = a.start[0], behind = a.start[a.requests];
+  }
+  __device__ __forceinline__ void arrived() { asm volatile("" : "+s"(before), "+s"(behind)); }
+  __device__ __forceinline__ void clear(const AttendArgs& a, int dim) {
+    if (__builtin_expect(before <= 0 && behind >= a.tokens, 1)) return;
+    before = min(max(before, 0), a.tokens), behind = min(max(behind, before), a.tokens);
+    const int64_t pieces = (int64_t)a.q_heads * dim / 8, first = before * pieces;
+    const int64_t all = (before + a.tokens - behind) * pieces, skip = (behind - before) * pieces;
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < all; i += (int64_t)gridDim.x * blockDim.x)
+      ((Vec<uint32_t, 4>*)a.out)[i < first ? i : i + skip] = Vec<uint32_t, 4>{};
+  }
+};
+
 // few rows: the wavefronts of a workgroup share them and split the keys; keys and values go
 // from memory into the registers they are multiplied from
 template <typename T, bool FP8, int D, int RT>
@@ -485,8 +505,10 @@ __global__ __launch_bounds__(kAttendWaves* kWave, D == 256 || RT == 2 ? 1 : 2) v
   const int lane = lane_id(), wave = threadIdx.x / kWave, c = lane & 15, j = lane >> 4;
   const int share = a.q_heads / a.kv_heads;
   const AttendUnit unit(a);
+  Rest rest(a);
   const int kv = unit.kv, chunk = unit.chunk, r = unit.r;
   const Request rq = request_of(a, r);
+  rest.arrived();
   const int rows = rq.queries * share;
   const int64_t bytes = (int64_t)a.block_size * D;  // of a block's head
   __shared__ float meet_top[kAttendWaves][ROWS], meet_sum[kAttendWaves][ROWS];
@@ -605,6 +627,7 @@ __global__ __launch_bounds__(kAttendWaves* kWave, D == 256 || RT == 2 ? 1 : 2) v
       __syncthreads();
     }
   }
+  rest.clear(a, D);
 }
 
 // many rows: each wavefront has its own, and the workgroup reads the keys and values once,
@@ -625,8 +648,10 @@ __global__ __launch_bounds__(kAttendWaves* kWave, D == 256 ? 1 : 2) void kv_atte
   const int lane = lane_id(), wave = threadIdx.x / kWave, c = lane & 15, j = lane >> 4;
   const int share = a.q_heads / a.kv_heads;
   const AttendUnit unit(a);
+  Rest rest(a);
   const int kv = unit.kv, chunk = unit.chunk, r = unit.r;
   const Request rq = request_of(a, r);
+  rest.arrived();
   const int rows = rq.queries * share;
   const int64_t bytes = (int64_t)a.block_size * D;
   // e4m3 codes stay codes in LDS: one instruction makes two elements of them.  int8 codes take
@@ -777,6 +802,7 @@ __global__ __launch_bounds__(kAttendWaves* kWave, D == 256 ? 1 : 2) void kv_atte
       }
     }
   }
+  rest.clear(a, D);
 }
 
 // brings the chunks of a row together: one wavefront per token and head
@@ -899,12 +925,11 @@ extern "C" int64_t ctmi_kv_attend_tmp_bytes(int64_t tokens, int64_t requests, in
   return l.most_chunks > 1 ? l.most_chunks * tokens * q_heads * (head_dim + 2) * 4 : 0;
 }
 
-extern "C" int ctmi_kv_attend(const void* q, int32_t dtype, int64_t q_token_stride, int64_t q_head_stride,
-                              void* out, int64_t tokens, int32_t q_heads, const ctmi_kv_blocks* blocks,
-                              const int32_t* block_table, int64_t table_stride, int64_t width,
-                              const int32_t* seq_lens, const int32_t* query_start, int64_t requests,
-                              float scale, int64_t max_query, int64_t max_seq, void* tmp,
-                              int64_t tmp_bytes, void* stream) {
+static int attend(bool clear, const void* q, int32_t dtype, int64_t q_token_stride, int64_t q_head_stride, void* out,
+                  int64_t tokens, int32_t q_heads, const ctmi_kv_blocks* blocks, const int32_t* block_table,
+                  int64_t table_stride, int64_t width, const int32_t* seq_lens, const int32_t* query_start,
+                  int64_t requests, float scale, int64_t max_query, int64_t max_seq, void* tmp, int64_t tmp_bytes,
+                  void* stream) {
   CTMI_REQUIRE(dtype == CTMI_BF16 || dtype == CTMI_F16, CTMI_ERR_UNSUPPORTED,
                "queries must be bfloat16 or float16");
   const int rc = check_kv_blocks(blocks);
@@ -944,7 +969,7 @@ extern "C" int ctmi_kv_attend(const void* q, int32_t dtype, int64_t q_token_stri
                blocks->block_size, q_heads, (int32_t)width, (int32_t)tokens, (int32_t)requests,
                (int32_t)l.tiles, (int32_t)l.chunks, (int32_t)l.chunk_keys, sixteenths,
                sixteenths == 1 ? 0u : (uint32_t)(((1ull << 32) + sixteenths - 1) / sixteenths),
-               scale * kLog2e};
+               scale * kLog2e, clear && query_start != nullptr};
   const hipStream_t s = (hipStream_t)stream;
   const dim3 blocks_of((unsigned)grid), threads(kAttendWaves * kWave);
   const bool fp8 = blocks->code_dtype == CTMI_F8E4M3;
@@ -967,4 +992,25 @@ extern "C" int ctmi_kv_attend(const void* q, int32_t dtype, int64_t q_token_stri
 #undef BY_CODE
 #undef BY_TILE
   return check_launch("kv_attend");
+}
+
+extern "C" int ctmi_kv_attend(const void* q, int32_t dtype, int64_t q_token_stride, int64_t q_head_stride,
+                              void* out, int64_t tokens, int32_t q_heads, const ctmi_kv_blocks* blocks,
+                              const int32_t* block_table, int64_t table_stride, int64_t width,
+                              const int32_t* seq_lens, const int32_t* query_start, int64_t requests,
+                              float scale, int64_t max_query, int64_t max_seq, void* tmp,
+                              int64_t tmp_bytes, void* stream) {
+  return attend(false, q, dtype, q_token_stride, q_head_stride, out, tokens, q_heads, blocks, block_table,
+                table_stride, width, seq_lens, query_start, requests, scale, max_query, max_seq, tmp, tmp_bytes, stream);
+}
+
+extern "C" int ctmi_kv_attend_padded(const void* q, int32_t dtype, int64_t q_token_stride, int64_t q_head_stride,
+                                     void* out, int64_t tokens, int32_t q_heads, const ctmi_kv_blocks* blocks,
+                                     const int32_t* block_table, int64_t table_stride, int64_t width,
+                                     const int32_t* seq_lens, const int32_t* query_start, int64_t requests,
+                                     float scale, int64_t max_query, int64_t max_seq, void* tmp,
+                                     int64_t tmp_bytes, void* stream) {
+  CTMI_REQUIRE(requests >= 1 || tokens < 1, CTMI_ERR_VALUE, "no request to take the rows of %lld tokens", (long long)tokens);
+  return attend(true, q, dtype, q_token_stride, q_head_stride, out, tokens, q_heads, blocks, block_table,
+                table_stride, width, seq_lens, query_start, requests, scale, max_query, max_seq, tmp, tmp_bytes, stream);
 }

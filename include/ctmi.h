@@ -797,6 +797,15 @@ int ctmi_kv_attend(const void* q, int32_t dtype, int64_t q_token_stride, int64_t
                    const int32_t* seq_lens, const int32_t* query_start, int64_t requests,
                    float scale, int64_t max_query, int64_t max_seq, void* tmp, int64_t tmp_bytes,
                    void* stream);
+/* The same, and the rows of tokens before query_start[0] and from query_start[requests] on become
+ * zeros, for an `out` that holds nothing yet (requests >= 1). */
+int ctmi_kv_attend_padded(const void* q, int32_t dtype, int64_t q_token_stride,
+                          int64_t q_head_stride, void* out, int64_t tokens, int32_t q_heads,
+                          const ctmi_kv_blocks* blocks, const int32_t* block_table,
+                          int64_t table_stride, int64_t width, const int32_t* seq_lens,
+                          const int32_t* query_start, int64_t requests, float scale,
+                          int64_t max_query, int64_t max_seq, void* tmp, int64_t tmp_bytes,
+                          void* stream);
 
 /* The bookkeeping of one serving step.  Request r holds seq_lens[r] tokens in the blocks
  * block_table[r, ...] names and gains new_tokens[r] >= 0, or ends (new_tokens[r] < 0): its

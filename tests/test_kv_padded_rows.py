@@ -1,0 +1,75 @@
+"""attend_kv_blocks without `out`: rows of tokens that belong to no request are zeros"""
+import pytest
+import torch
+
+from gpu_util import announce
+from test_kv_blocks import FP8, attention_case, check_attention, run_attention
+
+
+def poison(gpu, like):
+    """what the next allocation of that size may find: NaN everywhere"""
+    for _ in range(4):
+        keep = [torch.full_like(like, float("nan"), device=gpu) for _ in range(3)]
+        del keep
+    torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("codes,dtype", [(FP8, torch.bfloat16), (torch.int8, torch.float16)])
+@pytest.mark.parametrize("lens,news,size,dim,hints", [
+    ([40, 70], [2, 6], 16, 64, {}), ([40, 70], [1, 1], 64, 128, {"max_query": 1}), ([500], [200], 16, 128, {"max_query": 200}),
+    ([9000, 3], [1, 1], 64, 64, {"max_query": 1}), ([20, 20], [0, 0], 16, 256, {"max_query": 1}), ([3, 2], [2, 1], 32, 64, {"max_query": 90}),
+])
+@pytest.mark.parametrize("pad", [1, 30, 700])
+def test_rows_of_no_request_are_zeros(gpu, codes, dtype, lens, news, size, dim, hints, pad):
+    announce("padded rows", lens, news, size, dim, hints, pad, codes)
+    data = attention_case(lens, news, 8, 2, dim, size, codes, dtype, seed=1, pad=pad)
+    poison(gpu, data[0])
+    got = run_attention(gpu, *data, **hints)
+    assert (got[sum(news):] == 0).all()
+    check_attention(got, *data)
+    # and before the first request
+    q, cache, table, lens_t, starts = data
+    poison(gpu, q)
+    got = run_attention(gpu, q, cache, table, lens_t, starts + pad, **hints)
+    assert (got[:pad] == 0).all() and got.shape[0] == pad + sum(news)
+    check_attention(got, q, cache, table, lens_t, starts + pad)
+
+
+@pytest.mark.gpu
+def test_no_requests_and_steps_that_do_not_fit(gpu):
+    from compressed_tensors_amd.modeling import BlockKVCache, KVBlocks, attend_kv_blocks
+
+    q, cache, table, lens, _ = attention_case([5], [1], 4, 2, 64, 16, FP8, torch.bfloat16, pad=6)
+    poison(gpu, q)
+    on = KVBlocks(*(t.to(gpu) for t in cache))
+    none = torch.zeros(1, dtype=torch.int32, device=gpu)
+    got = attend_kv_blocks(q.to(gpu), on, table[:0].to(gpu), lens[:0].to(gpu), none)
+    assert got.shape == q.shape and (got == 0).all()
+    mark = torch.full_like(q, 3.0).to(gpu)
+    assert (attend_kv_blocks(q.to(gpu), on, table[:0].to(gpu), lens[:0].to(gpu), none, out=mark) == 3).all()
+
+    layer = BlockKVCache(1, 2, 2, 4, 1, 64, 16, device=gpu)
+    layer.plan(torch.tensor([20, 40], dtype=torch.int32, device=gpu), 60)  # 5 blocks of 2
+    x = torch.randn(60, 1, 64).bfloat16().to(gpu)
+    layer.update(0, x, x)
+    poison(gpu, x)
+    assert (layer.attend(0, x) == 0).all()
+
+
+@pytest.mark.gpu
+def test_rows_are_cleared_by_every_replay(gpu):
+    from compressed_tensors_amd.modeling import KVBlocks, attend_kv_blocks
+
+    q, cache, table, lens, starts = attention_case([100, 30], [1, 1], 8, 2, 64, 16, FP8, torch.bfloat16, pad=14)
+    on, q_d, table_d, lens_d, starts_d = KVBlocks(*(t.to(gpu) for t in cache)), *(t.to(gpu) for t in (q, table, lens, starts))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = attend_kv_blocks(q_d, on, table_d, lens_d, starts_d, max_query=1)
+    for now in ([0, 1, 2], [0, 1, 1], [0, 0, 0], [0, 3, 9]):
+        out.fill_(float("nan"))
+        starts_d.copy_(torch.tensor(now, dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert (out[now[-1]:] == 0).all()
+        check_attention(out, q, cache, table, lens, torch.tensor(now))
