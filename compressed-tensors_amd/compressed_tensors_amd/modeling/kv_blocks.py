@@ -178,8 +178,11 @@ def attend_kv_blocks(query: Tensor, blocks: KVBlocks, block_table: Tensor, seq_l
     i; one that sees none gives zeros.  q_heads is a multiple of the pool's heads: neighbouring
     query heads share one.  `softmax_scale` defaults to head_dim ** -0.5.
 
-    `max_query` and `max_seq`, the longest request's queries and keys, only choose the launch
-    (defaults: all tokens, the table's width); any values give the right result.  Rows of
+    `max_query` and `max_seq`, the longest request's queries and keys, choose the launch, and
+    with more than 64 queries x heads a kv head how many bits a softmax weight keeps on its way
+    into bfloat16 outputs (11, else 24); any values give the right result.  Without `max_query`
+    a batch of no more tokens than requests is taken for a decode step, any other for prompts;
+    `max_seq` defaults to the table's width.  Rows of
     tokens outside every request (a padded batch) keep what `out` holds; without `out` they are
     zeros.  Forward only."""
     c = _describe(blocks)
@@ -214,7 +217,10 @@ def attend_kv_blocks(query: Tensor, blocks: KVBlocks, block_table: Tensor, seq_l
         table_stride = width
     query = _aligned(query)
     longest = width * c.block_size
-    max_query = max(1, min(max_query, tokens)) if max_query is not None else 1 if query_start is None else max(1, tokens)
+    if max_query is None:
+        max_query = 1 if query_start is None else tokens + 1  # more than there are: not known
+    else:
+        max_query = max(1, min(max_query, tokens))
     max_seq = max(1, longest if max_seq is None else min(max_seq, longest))
     scale = dim ** -0.5 if softmax_scale is None else float(softmax_scale)
     lib = _lib.load()

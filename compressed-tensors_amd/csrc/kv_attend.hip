@@ -56,7 +56,7 @@ struct AttendArgs {
   float *part_o, *part_ml;  // [chunk][token][head][dim], [chunk][token][head][2]
   int64_t table_stride;
   int32_t num_blocks, kv_heads, block_size, q_heads, width, tokens, requests;
-  int32_t tiles, chunks, chunk_keys;  // of the grid
+  int32_t tiles, units, chunks, chunk_keys;  // of the grid: tiles of a request, or units of all and no tiles
   uint32_t sixteenths, magic;         // block_size / 16 and ceil(2^32 / that) (0: it is 1)
   float scale;                        // times log2(e)
   int32_t clear;                      // rows of no request become zeros
@@ -451,18 +451,44 @@ struct AttendRows {
   }
 };
 
-// what a workgroup works on, from its number
+// What a workgroup works on, from its number.  A request has a.tiles workgroups, or, where its
+// queries are not known (a.tiles is 0), one for its first tile, and for the further ones those from
+// start[r] * share / ROWS on: that leaves room for all of each request before it, and for one
+// more at times.  Whose a number is, the wavefront finds with 64 requests at a glance.
+// FIRST: first tiles come first (of a decode step there are no others), else last, as the rows
+// that see most do not lie in them.
+template <int ROWS, bool FIRST>
 struct AttendUnit {
+  static constexpr int kNone = 0x7FFFFFFF / ROWS;  // a tile behind those of any request
   int kv, chunk, tile, r;
-  __device__ __forceinline__ AttendUnit(const AttendArgs& a) {
+  __device__ __forceinline__ AttendUnit(const AttendArgs& a, int share) {
     int id = blockIdx.x;
     kv = id % a.kv_heads;
     id /= a.kv_heads;
     chunk = id % a.chunks;
     id /= a.chunks;
-    r = id % a.requests;
-    tile = a.tiles - 1 - id / a.requests;  // the rows that see most come first
+    if (a.tiles) {
+      r = id % a.requests;
+      tile = a.tiles - 1 - id / a.requests;  // the rows that see most come first
+      return;
+    }
+    const int unit = FIRST ? id : a.units - 1 - id;
+    r = unit, tile = 0;
+    if (unit < a.requests) return;
+    const int further = unit - a.requests;
+    auto first_of = [&](int q) { return (int)((uint32_t)min(max(a.start[q], 0), a.tokens) * (uint32_t)share / ROWS); };
+    int n = a.requests;
+    r = 0;
+    while (n > 1) {
+      const int step = (n + kWave - 1) / kWave, at = lane_id() * step;
+      const uint64_t begun = __ballot(at < n && first_of(r + min(at, n - 1)) <= further);
+      const int skip = max(__builtin_popcountll(begun) - 1, 0) * step;
+      r += skip, n = min(step, n - skip);
+    }
+    tile = further - first_of(r) + 1;
+    if (tile < 1) tile = kNone;
   }
+  __device__ __forceinline__ int next(const AttendArgs& a, int now) const { return a.tiles ? now + a.tiles : kNone; }
 };
 
 // the block of 16 keys from `key` on, and where in it they start
@@ -504,7 +530,7 @@ __global__ __launch_bounds__(kAttendWaves* kWave, D == 256 || RT == 2 ? 1 : 2) v
   constexpr int ROWS = RT * 16, CH = Rows::CH, DT = Rows::DT;
   const int lane = lane_id(), wave = threadIdx.x / kWave, c = lane & 15, j = lane >> 4;
   const int share = a.q_heads / a.kv_heads;
-  const AttendUnit unit(a);
+  const AttendUnit<ROWS, true> unit(a, share);
   Rest rest(a);
   const int kv = unit.kv, chunk = unit.chunk, r = unit.r;
   const Request rq = request_of(a, r);
@@ -514,7 +540,7 @@ __global__ __launch_bounds__(kAttendWaves* kWave, D == 256 || RT == 2 ? 1 : 2) v
   __shared__ float meet_top[kAttendWaves][ROWS], meet_sum[kAttendWaves][ROWS];
   __shared__ float meet_o[kAttendWaves][16][D + 4];
 
-  for (int tile = unit.tile; tile * ROWS < rows; tile += a.tiles) {
+  for (int tile = unit.tile; tile * ROWS < rows; tile = unit.next(a, tile)) {
     const int first = tile * ROWS, tile_end = last_key(rq, min(first + ROWS, rows) - 1, share);
     const int pieces = min(max((tile_end + a.chunk_keys - 1) / a.chunk_keys, 1), a.chunks);
     if (chunk >= pieces) continue;
@@ -647,7 +673,7 @@ __global__ __launch_bounds__(kAttendWaves* kWave, D == 256 ? 1 : 2) void kv_atte
   constexpr int KEYS = kAttendWaves * kWave / KP;                // keys per round of loads
   const int lane = lane_id(), wave = threadIdx.x / kWave, c = lane & 15, j = lane >> 4;
   const int share = a.q_heads / a.kv_heads;
-  const AttendUnit unit(a);
+  const AttendUnit<ROWS, false> unit(a, share);
   Rest rest(a);
   const int kv = unit.kv, chunk = unit.chunk, r = unit.r;
   const Request rq = request_of(a, r);
@@ -671,7 +697,7 @@ __global__ __launch_bounds__(kAttendWaves* kWave, D == 256 ? 1 : 2) void kv_atte
     }
   };
 
-  for (int tile = unit.tile; tile * ROWS < rows; tile += a.tiles) {
+  for (int tile = unit.tile; tile * ROWS < rows; tile = unit.next(a, tile)) {
     const int row0 = tile * ROWS, tile_end = last_key(rq, min(row0 + ROWS, rows) - 1, share);
     const int pieces = min(max((tile_end + a.chunk_keys - 1) / a.chunk_keys, 1), a.chunks);
     if (chunk >= pieces) continue;
@@ -873,14 +899,21 @@ constexpr Weights kRows = T::id == CTMI_F16 ? Weights::kPair : Weights::kHalf;
 struct Launch {
   bool split_keys;
   int row_tiles, tile_rows;
-  int64_t tiles, chunks, chunk_keys;
-  int64_t most_chunks;  // of any shorter max_seq, too
+  int64_t tiles, units, chunks, chunk_keys;
+  int64_t most_chunks;   // of any shorter max_seq, too
+  int64_t join_queries;  // a wavefront of the joining kernel has every so manyth query of a request
 };
 
-Launch plan_launch(int64_t requests, int32_t q_heads, int32_t kv_heads, int32_t head_dim, int64_t max_query,
-                   int64_t max_seq) {
+// A max_query above the tokens is one that the caller does not know.  No more tokens than requests
+// are then taken for a decode step, others for prompts, of which any may have all tokens (64
+// requests of 2500 keys, a token each: 58 us, as with hints; laid out for prompts 84).
+Launch plan_launch(int64_t tokens, int64_t requests, int32_t q_heads, int32_t kv_heads, int32_t head_dim,
+                   int64_t max_query, int64_t max_seq) {
+  constexpr int64_t kMost = 1 << 23;  // workgroups: a request of more tiles has each walk some
   Launch l;
-  const int64_t rows = max_query * (q_heads / kv_heads);
+  const bool known = max_query <= tokens;
+  const int64_t mean = cdiv(tokens, requests), share = q_heads / kv_heads;
+  const int64_t rows = (known ? max_query : mean == 1 ? 1 : tokens) * share;
   l.split_keys = rows <= 64;
   l.row_tiles = head_dim == 256 || rows <= 16 ? 1 : 2;
   l.tile_rows = (l.split_keys ? 1 : kAttendWaves) * l.row_tiles * 16;
@@ -907,6 +940,12 @@ Launch plan_launch(int64_t requests, int32_t q_heads, int32_t kv_heads, int32_t 
   l.chunks = cdiv(max_seq, l.chunk_keys);
   l.most_chunks = cdiv(max_seq, kFloor) < chunks ? cdiv(max_seq, kFloor) : chunks;
   if (l.split_keys && cdiv(max_seq, kLongest) > l.most_chunks) l.most_chunks = cdiv(max_seq, kLongest);
+  const int64_t most = kMost / (requests * l.chunks * kv_heads);
+  if (l.tiles > most) l.tiles = most < 1 ? 1 : most;
+  l.units = requests * l.tiles;
+  if (!known) l.tiles = 0, l.units = requests + tokens * share / l.tile_rows;
+  l.join_queries = known ? max_query : mean;
+  if (l.join_queries > kMost / (requests * q_heads)) l.join_queries = kMost / (requests * q_heads) < 1 ? 1 : kMost / (requests * q_heads);
   return l;
 }
 
@@ -919,9 +958,8 @@ extern "C" int64_t ctmi_kv_attend_tmp_bytes(int64_t tokens, int64_t requests, in
                                             int32_t kv_heads, int32_t head_dim, int64_t max_query,
                                             int64_t max_seq) {
   if (tokens < 1 || requests < 1 || q_heads < 1 || kv_heads < 1 || max_query < 1 || max_seq < 1) return 0;
-  if (max_query > tokens) max_query = tokens;
   if (max_seq > 1ll << 30) max_seq = 1ll << 30;
-  const Launch l = plan_launch(requests, q_heads, kv_heads, head_dim, max_query, max_seq);
+  const Launch l = plan_launch(tokens, requests, q_heads, kv_heads, head_dim, max_query, max_seq);
   return l.most_chunks > 1 ? l.most_chunks * tokens * q_heads * (head_dim + 2) * 4 : 0;
 }
 
@@ -951,23 +989,23 @@ static int attend(bool clear, const void* q, int32_t dtype, int64_t q_token_stri
   CTMI_REQUIRE(q_token_stride % 8 == 0 && q_head_stride % 8 == 0 && ((uintptr_t)q | (uintptr_t)out) % 16 == 0,
                CTMI_ERR_VALUE, "queries must be 16-byte aligned, token by token and head by head");
   const int32_t dim = blocks->head_dim;
-  if (max_query > tokens) max_query = tokens;
+  if (query_start == nullptr && max_query > tokens) max_query = 1;  // known after all; the same launch
   if (max_seq > width * blocks->block_size) max_seq = width * blocks->block_size > 0 ? width * blocks->block_size : 1;
-  const Launch l = plan_launch(requests, q_heads, blocks->kv_heads, dim, max_query, max_seq);
+  const Launch l = plan_launch(tokens, requests, q_heads, blocks->kv_heads, dim, max_query, max_seq);
   const int64_t cells = l.chunks > 1 ? l.chunks * tokens * q_heads : 0;
   CTMI_REQUIRE(tmp_bytes >= cells * (dim + 2) * 4 && (cells == 0 || (tmp != nullptr && (uintptr_t)tmp % 16 == 0)),
                CTMI_ERR_VALUE, "tmp needs %lld bytes at a 16-byte boundary, has %lld", (long long)(cells * (dim + 2) * 4),
                (long long)tmp_bytes);
-  const int64_t grid = requests * l.tiles * l.chunks * blocks->kv_heads;
-  const int64_t join = cdiv(requests * max_query * q_heads, (int64_t)kAttendWaves);
-  CTMI_REQUIRE(grid < (1ll << 31) && (cells == 0 || join < (1ll << 31)), CTMI_ERR_UNSUPPORTED, "too many requests and queries for one launch");
+  const int64_t grid = l.units * l.chunks * blocks->kv_heads;
+  const int64_t join = cdiv(requests * l.join_queries * q_heads, (int64_t)kAttendWaves);
+  CTMI_REQUIRE(grid < (1ll << 24) && (cells == 0 || join < (1ll << 24)), CTMI_ERR_UNSUPPORTED, "too many requests and heads for one launch");
   const uint32_t sixteenths = blocks->block_size / 16;
   AttendArgs a{(const uint16_t*)q, q_token_stride, q_head_stride, (uint16_t*)out,
                (const uint8_t*)blocks->key, (const uint8_t*)blocks->value, blocks->key_scale,
                blocks->value_scale, block_table, seq_lens, query_start, (float*)tmp,
                (float*)tmp + cells * dim, table_stride, (int32_t)blocks->num_blocks, blocks->kv_heads,
                blocks->block_size, q_heads, (int32_t)width, (int32_t)tokens, (int32_t)requests,
-               (int32_t)l.tiles, (int32_t)l.chunks, (int32_t)l.chunk_keys, sixteenths,
+               (int32_t)l.tiles, (int32_t)l.units, (int32_t)l.chunks, (int32_t)l.chunk_keys, sixteenths,
                sixteenths == 1 ? 0u : (uint32_t)(((1ull << 32) + sixteenths - 1) / sixteenths),
                scale * kLog2e, clear && query_start != nullptr};
   const hipStream_t s = (hipStream_t)stream;
@@ -982,7 +1020,7 @@ static int attend(bool clear, const void* q, int32_t dtype, int64_t q_token_stri
       kv_attend_rows_kernel<T, F, D, RT2, kRows<T>, false><<<blocks_of, threads, 0, s>>>(a);              \
     else if (RT2 == 1 || l.row_tiles == 1) kv_attend_split_kernel<T, F, D, 1><<<blocks_of, threads, 0, s>>>(a);    \
     else kv_attend_split_kernel<T, F, D, RT2><<<blocks_of, threads, 0, s>>>(a);                                    \
-    if (cells) kv_attend_join_kernel<T, D><<<dim3((unsigned)join), threads, 0, s>>>(a, l.tile_rows, (int)max_query); \
+    if (cells) kv_attend_join_kernel<T, D><<<dim3((unsigned)join), threads, 0, s>>>(a, l.tile_rows, (int)l.join_queries); \
   } while (0)
 #define BY_CODE(T, D) do { if (fp8) BY_TILE(T, true, D); else BY_TILE(T, false, D); } while (0)
 #define BY_DIM(T) do { if (dim == 64) BY_CODE(T, 64); else if (dim == 128) BY_CODE(T, 128); else BY_CODE(T, 256); } while (0)

@@ -786,8 +786,10 @@ int ctmi_kv_append(const void* key, const void* value, int32_t dtype, int64_t ke
  * elements), out [tokens, q_heads, head_dim] contiguous, of q's type; query head j reads kv
  * head j / (q_heads / kv_heads).  Tokens outside every request keep what `out` holds; a
  * block number outside the pool hides its positions.  max_query and max_seq (the longest
- * request's queries and keys, as far as the caller knows) only choose the launch: any
- * values give the same softmax.  tmp: ctmi_kv_attend_tmp_bytes bytes, 16-byte aligned. */
+ * request's queries and keys, as far as the caller knows; more queries than tokens: not known)
+ * choose the launch, and with it how many bits a weight of the softmax keeps on its way into a
+ * bf16 output: 24, or with more than 64 queries x heads a kv head 11.  Any values give the
+ * right result.  tmp: ctmi_kv_attend_tmp_bytes bytes, 16-byte aligned. */
 int64_t ctmi_kv_attend_tmp_bytes(int64_t tokens, int64_t requests, int32_t q_heads,
                                  int32_t kv_heads, int32_t head_dim, int64_t max_query,
                                  int64_t max_seq);
