@@ -96,7 +96,8 @@ class CompressedLinear(Linear):
             input.requires_grad or (self.bias is not None and self.bias.requires_grad))
         if (input.numel() <= _PACKED_ROWS * self.in_features and not differentiated
                 and input.dtype in (torch.bfloat16, torch.float16)):
-            return packed_linear(input, self.weight_packed, self.weight_scale, zero_point, self.bias)
+            # (loading a checkpoint makes scales that require grad; here, too, they are constants)
+            return packed_linear(input, self.weight_packed, self.weight_scale.detach(), zero_point, self.bias)
         weight = self.compressor.decompress_weight(
             {"weight_packed": self.weight_packed, "weight_scale": self.weight_scale, "weight_zero_point": zero_point,
              "weight_shape": (self.out_features, self.in_features)}, self.quantization_scheme.weights)

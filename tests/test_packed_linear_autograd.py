@@ -1,0 +1,49 @@
+"""CompressedLinear with keep_packed where autograd looks on: what it does not need differentiated
+takes the packed product, the rest the decompressed weight, nothing is dropped"""
+import pytest
+import torch
+
+from gpu_util import announce
+from test_packed_linear import check, make, packed_module
+
+
+def never(*args, **kwargs):
+    raise AssertionError("the weight was decompressed")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("symmetric,strategy", [(True, "group"), (False, "channel")])
+def test_scales_that_require_grad(gpu, symmetric, strategy, monkeypatch):
+    """parameters that a checkpoint's loading made: the scale of a module that stays packed is a constant,
+    as it is in a module that does not"""
+    announce("keep_packed, scale requires grad", symmetric, strategy)
+    module, packed, scale, zero, _ = packed_module(gpu, torch.bfloat16, symmetric, strategy, bias=False)
+    module.weight_scale = torch.nn.Parameter(module.weight_scale.data)
+    assert module.weight_scale.requires_grad
+    x = torch.randn(5, 256).bfloat16()
+    with torch.no_grad():
+        want = module(x.to(gpu))
+    monkeypatch.setattr(module.compressor, "decompress_weight", never)
+    got = module(x.to(gpu))
+    assert torch.equal(got, want) and not got.requires_grad
+    check(got, x, packed, scale, zero, None)
+
+
+@pytest.mark.gpu
+def test_scales_that_require_grad_beside_a_differentiated_input(gpu):
+    module, *_ = packed_module(gpu, torch.bfloat16, True, "group", bias=False)
+    dense = module.compressor.decompress_module(module)
+    module.weight_scale = torch.nn.Parameter(module.weight_scale.data)
+    x = torch.randn(3, 256).bfloat16().to(gpu).requires_grad_()
+    module(x).float().square().sum().backward()
+    other = x.detach().clone().requires_grad_()
+    torch.nn.functional.linear(other, dense).float().square().sum().backward()
+    assert torch.equal(x.grad, other.grad) and module.weight_scale.grad is None
+
+
+def test_scales_that_require_grad_are_not_refused():
+    """on the CPU the call gets as far as the kernel, which is on the GPU only"""
+    module, *_ = packed_module("cpu", torch.bfloat16, True, "group", bias=False)
+    module.weight_scale = torch.nn.Parameter(module.weight_scale.data)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        module(torch.randn(2, 256).bfloat16())
