@@ -38,6 +38,22 @@ def _frozen(data: Tensor) -> Parameter:
 _PACKED_ROWS = 192
 
 
+class _PackedProduct(torch.autograd.Function):
+    """packed_linear where nothing but the bias is differentiated"""
+
+    @staticmethod
+    def forward(input, weight_packed, weight_scale, weight_zero_point, bias):
+        return packed_linear(input, weight_packed, weight_scale, weight_zero_point, bias)
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        pass
+
+    @staticmethod
+    def backward(ctx, grad):
+        return None, None, None, None, grad.reshape(-1, grad.shape[-1]).sum(0)
+
+
 class CompressedLinear(Linear):
     #: multiply with the packed weight and never materialise it; set by `from_linear`
     keep_packed = False
@@ -92,12 +108,12 @@ class CompressedLinear(Linear):
         zero_point = getattr(self, "weight_zero_point", None)
         if self.quantization_scheme.weights.symmetric:
             zero_point = None
-        differentiated = torch.is_grad_enabled() and (
-            input.requires_grad or (self.bias is not None and self.bias.requires_grad))
-        if (input.numel() <= _PACKED_ROWS * self.in_features and not differentiated
-                and input.dtype in (torch.bfloat16, torch.float16)):
+        if (input.numel() <= _PACKED_ROWS * self.in_features and input.dtype in (torch.bfloat16, torch.float16)
+                and not (torch.is_grad_enabled() and input.requires_grad)):
             # (loading a checkpoint makes scales that require grad; here, too, they are constants)
-            return packed_linear(input, self.weight_packed, self.weight_scale.detach(), zero_point, self.bias)
+            learns = torch.is_grad_enabled() and self.bias is not None and self.bias.requires_grad
+            product = _PackedProduct.apply if learns else packed_linear
+            return product(input, self.weight_packed, self.weight_scale.detach(), zero_point, self.bias)
         weight = self.compressor.decompress_weight(
             {"weight_packed": self.weight_packed, "weight_scale": self.weight_scale, "weight_zero_point": zero_point,
              "weight_shape": (self.out_features, self.in_features)}, self.quantization_scheme.weights)

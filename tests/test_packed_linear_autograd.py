@@ -47,3 +47,31 @@ def test_scales_that_require_grad_are_not_refused():
     module.weight_scale = torch.nn.Parameter(module.weight_scale.data)
     with pytest.raises(RuntimeError, match="GPU only"):
         module(torch.randn(2, 256).bfloat16())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", [(256,), (1, 256), (40, 256), (2, 3, 256), (0, 256)])
+def test_a_bias_that_requires_grad_keeps_the_packed_product(gpu, dtype, shape, monkeypatch):
+    announce("keep_packed, bias requires grad", dtype, shape)
+    module, *_ = packed_module(gpu, dtype, False, "group")
+    assert module.bias.requires_grad  # as from_linear leaves it
+    x = torch.randn(shape).to(dtype).to(gpu)
+    with torch.no_grad():
+        want = module(x)
+    monkeypatch.setattr(module.compressor, "decompress_weight", never)
+    y = module(x)
+    assert torch.equal(y, want) and y.requires_grad
+    weight = torch.randn(y.shape).to(dtype).to(gpu)
+    for _ in range(2):  # gradients add up
+        (module(x) * weight).sum().backward()
+    # a sum of m numbers in fp32, rounded once, twice over: half a step each, and of their sum
+    exact = 2 * weight.double().reshape(-1, 96).sum(0)
+    spread = weight.double().reshape(-1, 96).abs().sum(0)
+    bound = torch.finfo(dtype).eps * 1.5 * exact.abs() + 2 * 40 * 2.0 ** -24 * spread
+    assert module.bias.grad.dtype is dtype and ((module.bias.grad.double() - exact).abs() <= bound).all()
+    # ... and its own gradient: the sum is linear
+    v = torch.ones(96, dtype=dtype, device=gpu, requires_grad=True)
+    grad, = torch.autograd.grad(module(x), module.bias, v.expand(y.shape), create_graph=True)
+    again, = torch.autograd.grad(grad.sum(), v)
+    assert (again == weight.reshape(-1, 96).shape[0]).all()
