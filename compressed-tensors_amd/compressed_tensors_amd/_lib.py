@@ -13,6 +13,7 @@ from pathlib import Path
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 import os
 
@@ -498,6 +499,25 @@ def ptr(t: Optional[torch.Tensor]) -> Optional[int]:
 # torch's own shortcut to the current stream's handle (what its compiled kernels' launchers
 # call): a tenth of the cost of building a torch.cuda.Stream object on every library call
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def has_tangent(*tensors: Optional[torch.Tensor]) -> bool:
+    """whether one of the tensors is a dual one of forward-mode differentiation (which does not
+    require grad, and carries its tangent through no_grad)"""
+    if getattr(forward_ad, "_current_level", 0) >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                return True
+    return False
+
+
+def differentiated(*tensors: Optional[torch.Tensor]) -> bool:
+    """whether autograd follows one of the tensors, backward or forward"""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return has_tangent(*tensors)
 
 
 def gpu_index(first: torch.Tensor, *others: Optional[torch.Tensor]) -> int:

@@ -19,6 +19,7 @@ from torch import Tensor
 from torch.nn import Linear, Parameter
 from torch.nn import functional as F
 
+from compressed_tensors_amd import _lib
 from compressed_tensors_amd.compressors.base import BaseCompressor
 from compressed_tensors_amd.config import CompressionFormat, QuantizationStatus
 from compressed_tensors_amd.linear.packed import packed_linear
@@ -109,7 +110,7 @@ class CompressedLinear(Linear):
         if self.quantization_scheme.weights.symmetric:
             zero_point = None
         if (input.numel() <= _PACKED_ROWS * self.in_features and input.dtype in (torch.bfloat16, torch.float16)
-                and not (torch.is_grad_enabled() and input.requires_grad)):
+                and not _lib.differentiated(input) and not _lib.has_tangent(self.bias)):
             # (loading a checkpoint makes scales that require grad; here, too, they are constants)
             learns = torch.is_grad_enabled() and self.bias is not None and self.bias.requires_grad
             product = _PackedProduct.apply if learns else packed_linear

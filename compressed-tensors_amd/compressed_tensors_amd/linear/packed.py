@@ -48,10 +48,9 @@ def packed_linear(x: Tensor, weight_packed: Tensor, weight_scale: Tensor,
         raise ValueError(f"{k} columns need {(k + 7) // 8} words a row, weight_packed has {weight_packed.shape[1]}")
     if weight_scale.shape[0] != n or groups < 1 or k % groups:
         raise ValueError(f"scales {tuple(weight_scale.shape)} do not fit a [{n}, {k}] weight")
-    if torch.is_grad_enabled() and (x.requires_grad or weight_scale.requires_grad
-                                    or (bias is not None and bias.requires_grad)):
-        raise NotImplementedError("packed_linear has no backward: decompress the weight to differentiate, "
-                                  "or call it under torch.no_grad()")
+    if _lib.differentiated(x, weight_scale, bias):
+        raise NotImplementedError("packed_linear has no backward and no forward-mode derivative: decompress the "
+                                  "weight to differentiate, or call it under torch.no_grad() with plain tensors")
     if weight_zero_point is not None:
         if weight_zero_point.dtype is not torch.int32 or tuple(weight_zero_point.shape) != ((n + 7) // 8, groups):
             raise ValueError(f"expected packed zero points int32 [{(n + 7) // 8}, {groups}], got "

@@ -144,8 +144,9 @@ def append_kv_blocks(key: Tensor, value: Tensor, blocks: KVBlocks, slots: Tensor
                          f"{tuple(key.shape)} and {tuple(value.shape)}")
     if key.dtype not in _INPUTS or value.dtype is not key.dtype:
         raise NotImplementedError(f"keys and values must be bfloat16 or float16, got {key.dtype} and {value.dtype}")
-    if torch.is_grad_enabled() and (key.requires_grad or value.requires_grad):
-        raise NotImplementedError("append_kv_blocks has no backward: call it under torch.no_grad()")
+    if _lib.differentiated(key, value):
+        raise NotImplementedError("append_kv_blocks has no backward and no forward-mode derivative: call it under "
+                                  "torch.no_grad() with plain tensors")
     slots = _ints("slots", slots, torch.int64, key.shape[0])
     index = _lib.gpu_index(key, value, slots, *blocks)
     if not _lib.is_current(index):
@@ -190,8 +191,9 @@ def attend_kv_blocks(query: Tensor, blocks: KVBlocks, block_table: Tensor, seq_l
         raise ValueError(f"expected queries [tokens, a multiple of {c.kv_heads}, {c.head_dim}], got {tuple(query.shape)}")
     if query.dtype not in _INPUTS:
         raise NotImplementedError(f"queries must be bfloat16 or float16, got {query.dtype}")
-    if torch.is_grad_enabled() and query.requires_grad:
-        raise NotImplementedError("attend_kv_blocks has no backward: call it under torch.no_grad()")
+    if _lib.differentiated(query):
+        raise NotImplementedError("attend_kv_blocks has no backward and no forward-mode derivative: call it under "
+                                  "torch.no_grad() with plain tensors")
     lens = _ints("seq_lens", seq_lens, torch.int32)
     requests, (tokens, heads, dim) = lens.shape[0], query.shape
     if block_table.dtype is not torch.int32 or block_table.ndim != 2 or block_table.shape[0] != requests:

@@ -75,3 +75,40 @@ def test_a_bias_that_requires_grad_keeps_the_packed_product(gpu, dtype, shape, m
     grad, = torch.autograd.grad(module(x), module.bias, v.expand(y.shape), create_graph=True)
     again, = torch.autograd.grad(grad.sum(), v)
     assert (again == weight.reshape(-1, 96).shape[0]).all()
+
+
+def test_dual_tensors_are_refused():
+    """forward-mode derivatives: a call that would drop a tangent raises, with and without no_grad"""
+    from torch.autograd import forward_ad
+
+    from compressed_tensors_amd.linear import packed_linear
+
+    x, packed, scale, _, bias = make(2, 16, 128, 2, torch.bfloat16, bias=True)
+    with forward_ad.dual_level():
+        for i in range(3):
+            args = [x, scale, bias]
+            args[i] = forward_ad.make_dual(args[i], torch.ones_like(args[i]))
+            for mode in (torch.enable_grad(), torch.no_grad()):
+                with mode, pytest.raises(NotImplementedError, match="forward-mode"):
+                    packed_linear(args[0], packed, args[1], None, args[2])
+        with pytest.raises(RuntimeError, match="GPU only"):  # plain tensors inside a level
+            packed_linear(x, packed, scale, None, bias)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("grad", [True, False])
+def test_dual_tensors_go_through_the_decompressed_weight(gpu, grad):
+    from torch.autograd import forward_ad
+
+    module, *_ = packed_module(gpu, torch.bfloat16, True, "group")
+    dense = module.compressor.decompress_module(module)
+    x, t = torch.randn(3, 256).bfloat16().to(gpu), torch.randn(3, 256).bfloat16().to(gpu)
+    bias, bt = module.bias.detach(), torch.randn(96).bfloat16().to(gpu)
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+        got = forward_ad.unpack_dual(module(forward_ad.make_dual(x, t)))
+        want = forward_ad.unpack_dual(torch.nn.functional.linear(forward_ad.make_dual(x, t), dense, bias))
+        assert torch.equal(got.primal, want.primal) and torch.equal(got.tangent, want.tangent)
+        del module.bias
+        module.bias = forward_ad.make_dual(bias, bt)
+        got = forward_ad.unpack_dual(module(x))
+        assert torch.equal(got.tangent, bt.expand(3, 96))
