@@ -13,6 +13,7 @@ remains a quarter of the dense one's size, a forward call of few rows multiplies
 codes (`packed_linear`), and one of many rows decompresses the weight for that call.
 """
 import warnings
+from typing import Optional
 
 import torch
 from torch import Tensor
@@ -79,7 +80,9 @@ class CompressedLinear(Linear):
         keep_packed: see the module's description; `pack-quantized` weights of 4 bits with
         groups of a multiple of 32 columns or one scale per row, no activation ordering."""
         if keep_packed:
-            _check_keeps_packed(module, quantization_scheme.weights, quantization_format)
+            reason = why_not_kept_packed(module, quantization_scheme.weights, quantization_format)
+            if reason is not None:
+                raise NotImplementedError(reason)
         compressor = BaseCompressor.load_from_registry(quantization_format)
         dense_shape, device = module.weight.shape, module.weight.device
 
@@ -128,15 +131,16 @@ class CompressedLinear(Linear):
         return F.linear(input, self.weight, self.bias)
 
 
-def _check_keeps_packed(module: Linear, args, quantization_format: str) -> None:
-    """refuse what the product with packed weights does not read"""
+def why_not_kept_packed(module: Linear, args, quantization_format: str) -> Optional[str]:
+    """what keeps the product with packed weights from reading this one; None: nothing does"""
     if quantization_format != CompressionFormat.pack_quantized.value or args is None or args.num_bits != 4 or args.type != "int":
-        raise NotImplementedError("keep_packed needs a pack-quantized 4-bit integer weight")
+        return "keep_packed needs a pack-quantized 4-bit integer weight"
     if getattr(args, "actorder", None) is not None and str(getattr(args.actorder, "value", args.actorder)) == "group":
-        raise NotImplementedError("keep_packed does not take weights with activation ordering")
+        return "keep_packed does not take weights with activation ordering"
     strategy = str(getattr(args.strategy, "value", args.strategy))
     if strategy == "group" and args.group_size % 32 == 0 and module.in_features % args.group_size == 0:
-        return
+        return None
     if strategy != "channel":
-        raise NotImplementedError(f"keep_packed needs one scale per row or groups of a multiple of 32 columns that "
-                                  f"divide {module.in_features}, got {strategy} {args.group_size}")
+        return (f"keep_packed needs one scale per row or groups of a multiple of 32 columns that divide "
+                f"{module.in_features}, got {strategy} {args.group_size}")
+    return None

@@ -11,6 +11,7 @@ Matching of targets is by module name, class name or `re:` expression
 (utils/match.py:40-100); the first target of the config that matches a module decides
 its scheme.
 """
+import warnings
 from collections import OrderedDict
 from copy import deepcopy
 from typing import Generator, Optional, Tuple
@@ -90,9 +91,11 @@ def apply_quantization_config(model: Module, config: Optional[QuantizationConfig
     """attach the schemes of `config` to the modules they target and give these their
     scales and zero points (initialize_module_for_quantization); with run_compressed and a
     format other than dense a Linear becomes a CompressedLinear that holds the compressed
-    parameters, and with keep_packed one that multiplies with them as they are (4-bit
-    pack-quantized weights).  A kv_cache_scheme goes onto every attention module."""
-    from compressed_tensors_amd.linear.compressed_linear import CompressedLinear
+    parameters, and with keep_packed one that multiplies with them as they are where that can
+    be done (4-bit pack-quantized weights, CompressedLinear.from_linear); a warning names what
+    cannot, which decompresses as without keep_packed.  A kv_cache_scheme goes onto every
+    attention module."""
+    from compressed_tensors_amd.linear.compressed_linear import CompressedLinear, why_not_kept_packed
     from compressed_tensors_amd.modeling import initialize_hooked_attention, initialize_hooked_kv_cache
 
     config = deepcopy(config)
@@ -116,18 +119,25 @@ def apply_quantization_config(model: Module, config: Optional[QuantizationConfig
 
     # a target that names no module is worth a warning; of several targets that name a module
     # the most specific decides: its name, then a pattern, then a class (apply.py:140-160)
+    not_kept = {}
     for name, module in list(match_named_modules(model, target_to_scheme, config.ignore, warn_on_fail=True)):
         scheme = target_to_scheme[match_targets(name, module, target_to_scheme)[0]]
         module.quantization_scheme = scheme
         if (run_compressed and isinstance(module, torch.nn.Linear)
                 and config.format != CompressionFormat.dense.value):
+            reason = why_not_kept_packed(module, scheme.weights, config.format) if keep_packed else None
+            if reason is not None:
+                not_kept.setdefault(reason, []).append(name)
             CompressedLinear.from_linear(module, quantization_scheme=scheme, quantization_format=config.format,
-                                         keep_packed=keep_packed)
+                                         keep_packed=keep_packed and reason is None)
         else:
             if is_attention_module(module) and is_narrow_match(model, scheme.targets, name):
                 initialize_hooked_attention(model, module)
             initialize_module_for_quantization(module, force_zero_point=force_zero_point)
         module.quantization_status = status
+    for reason, names in not_kept.items():
+        more = f" and {len(names) - 1} more" if len(names) > 1 else ""
+        warnings.warn(f"{names[0]}{more} will not stay packed: {reason}", UserWarning, stacklevel=2)
 
 
 def load_pretrained_quantization_parameters(model: Module, model_name_or_path: Optional[str] = None,
