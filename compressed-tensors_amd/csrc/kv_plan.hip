@@ -67,7 +67,7 @@ struct PlanRequest {
     held = len / bs + (len % bs != 0);
     const uint32_t after = len + add;
     need = after / bs + (after % bs != 0);
-    fits = l >= 0 && need <= (uint32_t)a.width && held <= (uint32_t)a.width;
+    fits = l >= 0 && after <= 0x7FFFFFFFu && need <= (uint32_t)a.width && held <= (uint32_t)a.width;
   }
 };
 

@@ -821,7 +821,7 @@ int ctmi_kv_attend_padded(const void* q, int32_t dtype, int64_t q_token_stride,
  *   free_out [free_capacity], num_free_out [1]   the stack afterwards, -1 behind
  *   status [1]: 0, or the step did not fit and every output equals its input, slots -1 and
  *     query_start 0: > 0 that many blocks are missing; -1 a request does not fit its table
- *     row (or has a negative length); -2 more than slot_count new tokens; -3 the free list
+ *     row (or its length is negative, or would not stay below 2^31); -2 more than slot_count new tokens; -3 the free list
  *     does not hold what it should (num_free outside 0 ... free_capacity, or more blocks
  *     come back than fit). */
 int ctmi_kv_plan(const int32_t* seq_lens, const int32_t* new_tokens, const int32_t* block_table,
