@@ -112,12 +112,18 @@ class CompressedLinear(Linear):
         zero_point = getattr(self, "weight_zero_point", None)
         if self.quantization_scheme.weights.symmetric:
             zero_point = None
-        if (input.numel() <= _PACKED_ROWS * self.in_features and input.dtype in (torch.bfloat16, torch.float16)
-                and not _lib.differentiated(input) and not _lib.has_tangent(self.bias)):
+        bias = self.bias
+        # (what F.linear casts to inside autocast, and what it does not)
+        cast = torch.is_autocast_enabled("cuda") and input.dtype is not torch.float64
+        dtype = torch.get_autocast_dtype("cuda") if cast else input.dtype
+        if (input.numel() <= _PACKED_ROWS * self.in_features and dtype in (torch.bfloat16, torch.float16)
+                and not _lib.differentiated(input) and not _lib.has_tangent(bias)):
+            if cast:
+                input, bias = input.to(dtype), None if bias is None else bias.to(dtype)
             # (loading a checkpoint makes scales that require grad; here, too, they are constants)
-            learns = torch.is_grad_enabled() and self.bias is not None and self.bias.requires_grad
+            learns = bias is not None and bias.requires_grad and torch.is_grad_enabled()
             product = _PackedProduct.apply if learns else packed_linear
-            return product(input, self.weight_packed, self.weight_scale.detach(), zero_point, self.bias)
+            return product(input, self.weight_packed, self.weight_scale.detach(), zero_point, bias)
         weight = self.compressor.decompress_weight(
             {"weight_packed": self.weight_packed, "weight_scale": self.weight_scale, "weight_zero_point": zero_point,
              "weight_shape": (self.out_features, self.in_features)}, self.quantization_scheme.weights)

@@ -112,3 +112,26 @@ def test_dual_tensors_go_through_the_decompressed_weight(gpu, grad):
         module.bias = forward_ad.make_dual(bias, bt)
         got = forward_ad.unpack_dual(module(x))
         assert torch.equal(got.tangent, bt.expand(3, 96))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("given", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("cast", [torch.bfloat16, torch.float16])
+def test_autocast(gpu, given, cast, monkeypatch):
+    """inside autocast the product is one in autocast's type, whatever input and bias are, as that
+    of a module that does not stay packed"""
+    module, packed, scale, zero, _ = packed_module(gpu, torch.bfloat16, True, "group")
+    module.bias.data = module.bias.data.float()
+    dense = module.compressor.decompress_module(module)
+    x = torch.randn(6, 256)
+    x = x.to(given)
+    with torch.autocast("cuda", dtype=cast):
+        ordinary = torch.nn.functional.linear(x.to(gpu), dense, module.bias)
+        monkeypatch.setattr(module.compressor, "decompress_weight", never)
+        with torch.no_grad():
+            got = module(x.to(gpu))
+        y = module(x.to(gpu))
+    assert got.dtype is ordinary.dtype is cast and torch.equal(y, got)
+    check(got, x.to(cast), packed, scale, zero, module.bias.detach().cpu().to(cast))
+    y.sum().backward()
+    assert module.bias.grad.dtype is torch.float32 and (module.bias.grad == 6).all()
