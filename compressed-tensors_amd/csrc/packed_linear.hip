@@ -646,6 +646,10 @@ LinearLaunch plan_linear(int64_t m, int64_t n, int64_t k) {
   l.splits = 1;
   if (m <= 16 || k % 32 != 0) {
     l.mt = 1;
+    // Wide enough to fill the device, a wavefront takes more tiles: x and its sums serve more columns.
+    // Of k 4096, one row (16 rows), 1, 2 and 4 tiles: 4096 columns 6.2, 7.2, 11.0 us (7.2, 8.4, 12.3);
+    // 8192 9.1, 7.8, 11.2 (11.0, 8.8, 12.7); 16384 14.8, 11.6, 11.8 (18.0, 13.6, 13.8); 28672 23.8, 19.0,
+    // 16.2 (28.1, 22.5, 20.0).
     l.nt = tiles >= 1024 ? 4 : tiles >= 512 ? 2 : 1;
     l.waves = l.nt == 4 ? 4 : 8;
     l.wave_k = cdiv(cdiv(k, l.waves), kStepK) * kStepK;
@@ -654,7 +658,9 @@ LinearLaunch plan_linear(int64_t m, int64_t n, int64_t k) {
     l.nt = 2;
     l.waves = 8;
     // one workgroup per compute unit; a split's sums leave and come back in fp32, so no more
-    // of them than it takes, of 256 columns at least
+    // of them than it takes, of 256 columns at least.  Not above 16: 64 x 1024 x 14336 takes 23.2,
+    // 19.9 and 22.2 us with up to 8, 16 and 32, 32 x 1024 x 14336 17.7, 16.0 and 17.8 (of 28672
+    // columns 34.1, 26.1 and 24.8).
     const int64_t units = cdiv(tiles, 8) * cdiv(m, l.mt * 16);
     if (units < 256) l.splits = 256 / units;
     if (l.splits > k / 512) l.splits = k / 512 > 0 ? k / 512 : 1;

@@ -1,8 +1,9 @@
 """What attend_kv_blocks keeps of a softmax weight on its way into the second product.
 
 Tolerance: a score's sum, the exponential and the additions as in test_kv_blocks (relative to
-sum p |v|), and the weights.  With at most 64 rows a kv head, and for float16 outputs, these are
-two or more bf16 numbers: 2^-16.  For bf16 outputs of more rows one f16 number for weight times
+sum p |v|), and the weights.  With at most 64 rows a kv head these are three bf16 numbers, which
+hold all 24 bits (each leaves at most 2^-8 of what it rounds): 2^-24.  For float16 outputs of more
+rows two: 2^-16.  For bf16 outputs of more rows one f16 number for weight times
 scale, the largest being 2^7 or more: half a step, eps / 2 = 2^-11, and where f16 has no finer
 steps half its smallest, 2^-25, which is 2^-32 of the largest weight times scale, for each key and
 as many times as its code says.  Where the sum below is of the same numbers their scale is no less
@@ -16,12 +17,13 @@ from oracle import serving as osv
 from test_kv_blocks import FP8, attention_case, run_attention
 
 
-def check(got, q, cache, table, lens, starts, rows, single, keys, steepest):
-    """single: weights are one number; keys: how many of them have a value, steepest: by how much
+def check(got, q, cache, table, lens, starts, rows, many, keys, steepest):
+    """many: more than 64 rows a kv head; keys: how many of them have a value, steepest: by how much
     a value may exceed the sum of p |v| that it is part of"""
+    single = many and got.dtype is torch.bfloat16
     want, mag, reach = (t[rows] for t in osv.kv_attend(q, cache, table, lens, starts))
     n, eps = int(max(lens)), torch.finfo(got.dtype).eps
-    weight = 2.0 ** -11 + n * 2.0 ** -24 if single else 2.0 ** -16
+    weight = 2.0 ** -11 + n * 2.0 ** -24 if single else 2.0 ** -16 if many else 2.0 ** -24
     rel = weight + 2.0 ** -20 + 2 * (q.shape[2] / 32 + 40) * 2.0 ** -24 * reach + (n / 32 + 96) * 2.0 ** -24
     low = keys * 2.0 ** -32 * steepest if single else 0.0
     bound = (eps / 2 + 1.004 * weight) * want.abs() + rel * mag + low * mag.amax(dim=2, keepdim=True)
@@ -58,7 +60,7 @@ def test_weights_of_values_that_cancel(gpu, dtype, codes, news, size):
             p = torch.softmax((k @ q[-1, h * share].double()) * 0.125, 0)
             cache[3][last, h] = float(p[0] * 96.0 * 0.03125 / (p[-1] * 112.0))
         got = run_attention(gpu, *data, max_query=q.shape[0])
-        check(got, *data, slice(-1, None), dtype is torch.bfloat16 and q.shape[0] * share > 64, 2, 1)
+        check(got, *data, slice(-1, None), q.shape[0] * share > 64, 2, 1)
 
 
 SPREADS = {"rising": lambda i: 2.0 ** (i * 3 - 30), "falling": lambda i: 2.0 ** (25 - 3 * i), "one huge": lambda i: 1e6 if i == 2 else 0.01,
@@ -82,7 +84,7 @@ def test_scales_of_values_far_apart(gpu, dtype, codes, spread, news, size):
         cache[3].clamp_(-1.0, 1.0)
     got = run_attention(gpu, *data, max_query=news)
     # the key with the largest weight times scale has a code of more than 90 among its 64
-    check(got, *data, slice(None), dtype is torch.bfloat16 and news * 2 > 64, 300, 448 / 90)
+    check(got, *data, slice(None), news * 2 > 64, 300, 448 / 90)
 
 
 @pytest.mark.gpu
