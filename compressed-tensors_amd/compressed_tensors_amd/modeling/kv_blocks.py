@@ -182,8 +182,9 @@ def attend_kv_blocks(query: Tensor, blocks: KVBlocks, block_table: Tensor, seq_l
     `max_query` and `max_seq`, the longest request's queries and keys, choose the launch, and
     with more than 64 queries x heads a kv head how many bits a softmax weight keeps on its way
     into bfloat16 outputs (11, else 24); any values give the right result.  Without `max_query`
-    a batch of no more tokens than requests is taken for a decode step, any other for prompts;
-    `max_seq` defaults to the table's width.  Rows of
+    a batch of no more tokens than requests is taken for a decode step, any other for prompts,
+    and a batch of very different requests is better left without it; `max_seq` defaults to the
+    table's width.  Rows of
     tokens outside every request (a padded batch) keep what `out` holds; without `out` they are
     zeros.  Forward only."""
     c = _describe(blocks)

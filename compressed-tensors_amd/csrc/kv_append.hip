@@ -11,8 +11,9 @@
 // whose result is the same for finite x and scales within 2^+-100.  A run that holds anything
 // else, or values beyond 2^16 scales (which scales given by the caller allow), divides.
 //
-// Measured on one MI355X, 8 heads of 128: 3 prompts of 4001 tokens (67 MB) 21 us, 3.1 TB/s with
-// the vector units 61 % busy, which is what bounds it; one token for each of 48 requests 5 us.
+// Measured on one MI355X, 8 heads of 128: 3 prompts of 4001 tokens (67 MB) 21 us, 3.2 TB/s, with
+// the vector units 57 % busy and wavefronts waiting 27 % of their time: neither alone bounds it;
+// one token for each of 48 requests 5.5 us.
 //
 // Keys: a thread encodes 4 neighbouring dimensions of a token and stores a word.  Values lie
 // transposed, tokens innermost: a thread takes 4 dimensions of the 4 tokens that share a word

@@ -25,8 +25,8 @@
 // and weights meet in a second, small kernel.
 //
 // Measured on one MI355X, 32 heads over 8 of 128 dimensions: one token for each of 64 requests
-// of up to 4096, 82 us, 5.5 TB/s (memory bounds it); 6 of up to 32768, 77 us, 5.0 TB/s, and 5 us
-// for the parts; 2 prompts of 2000 over 4000 keys 252 us, 0.71 PFLOP/s, vector units 55 % and
+// of up to 4096, 83 us, 5.4 TB/s (memory bounds it); 6 of up to 32768, 77 us, 5.0 TB/s, and 5 us
+// for the parts; 2 prompts of 2000 over 4000 keys 259 us, 0.69 PFLOP/s, vector units 55 % and
 // matrix cores 31 % busy: the softmax between the products bounds it.
 #include <type_traits>
 
