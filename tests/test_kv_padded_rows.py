@@ -73,3 +73,38 @@ def test_rows_are_cleared_by_every_replay(gpu):
         torch.cuda.synchronize()
         assert (out[now[-1]:] == 0).all()
         check_attention(out, q, cache, table, lens, torch.tensor(now))
+
+
+@pytest.mark.gpu
+def test_calls_on_two_streams(gpu):
+    """two batches without hints at once, each on a stream of its own"""
+    from compressed_tensors_amd.modeling import KVBlocks, attend_kv_blocks
+
+    batches = []
+    for seed, (lens, news) in enumerate((([900, 70, 1], [1, 1, 1]), ([300, 40], [150, 3]))):
+        q, cache, table, lens, starts = attention_case(lens, news, 8, 2, 64, 32, FP8, torch.bfloat16, seed=seed, pad=4)
+        args = (q.to(gpu), KVBlocks(*(t.to(gpu) for t in cache)), table.to(gpu), lens.to(gpu), starts.to(gpu))
+        batches.append((args, attend_kv_blocks(*args), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(10):
+        for args, _, stream in batches:
+            with torch.cuda.stream(stream):
+                got.append(attend_kv_blocks(*args))
+    torch.cuda.synchronize()
+    for i, out in enumerate(got):
+        assert torch.equal(out, batches[i % 2][1])
+
+
+def test_abi_refusals(ctmi):
+    from ctypes import byref
+
+    from compressed_tensors_amd._lib import KVBlocksC
+
+    def attend(requests=2, tokens=3, start=16, max_query=1, heads=4, stride=128):
+        return ctmi.ctmi_kv_attend_padded(16, 2, stride, 64, 16, tokens, heads, byref(KVBlocksC(16, 16, 16, 16, 4, 2, 64, 16, 3)), 16, 3, 3,
+                                          16, start, requests, 0.1, max_query, 48, None, 0, None)
+
+    assert attend(requests=0) == -1  # nothing says which rows are whose
+    assert attend(requests=0, tokens=0) == 0 and attend(tokens=0) == 0
+    assert attend(start=None) == -1 and attend(max_query=0) == -1 and attend(heads=3) == -1 and attend(stride=100) == -1
